@@ -178,7 +178,7 @@ def _free_stack(pages):
 
 def _tables(seqs, max_ctx, pages, max_rows):
     z = lambda *s: torch.zeros(s, dtype=torch.int32, device=DEV)
-    return dict(block_table=z(seqs, max(1, _pages(max_ctx))), held=z(seqs), free=_free_stack(pages),
+    return dict(block_table=z(seqs, max(1, _pages(max_ctx))), held=z(seqs), free_pages=_free_stack(pages),
                 n_free=torch.full((1,), pages, dtype=torch.int32, device=DEV), row_start=z(seqs + 1),
                 kv_start=z(seqs + 1), slot=z(max_rows), pos=z(max_rows), row_seq=z(max_rows), status=z(1))
 
@@ -197,7 +197,7 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-TABLES = ("block_table", "held", "free", "n_free", "row_start", "kv_start", "slot", "pos", "row_seq", "status")
+TABLES = ("block_table", "held", "free_pages", "n_free", "row_start", "kv_start", "slot", "pos", "row_seq", "status")
 
 
 def prepare(case, seed):
@@ -217,13 +217,14 @@ def prepare(case, seed):
     pre = np.minimum(ctx, 1) if op == "plan" else ctx
     max_rows = max(T, int(pre.sum()))
     if op == "plan":
-        st.update(kv_heads=1, head_dim=32, kv="int8")
+        st.update(kv_heads=1, head_dim=32, kv="int8", dtype="f32")
         st["drop"] = dev(np.full(B, -1))
     if own:
         flb200, lib = _lib()
         st["kv8"] = flb200.KV8Cache(lib, layers=1, heads=st.get("heads", st["kv_heads"]), kv_heads=st["kv_heads"],
                                     head_dim=st["head_dim"], pages=pages, max_seqs=B, max_rows=max_rows,
-                                    max_ctx=max_ctx, type=st["kv"], device=torch.cuda.current_device())
+                                    max_ctx=max_ctx, type=st["kv"], dtype=str(DTYPES[st["dtype"]])[6:],
+                                    device=torch.cuda.current_device())
         t = st["kv8"].tables()
         st["tables"] = {n: torch.as_tensor(t[n], device=DEV) for n in TABLES}
     else:
@@ -352,7 +353,7 @@ def _plan_pages(t, need, drop):
     nrel, ntake = rel.sum(), take.sum()
     ok = (ntake <= n_free + nrel)[0] & (need.max() <= mp)
     # release: the first page of the first sequence ends on top
-    free = torch.cat([t["free"], t["free"].new_zeros(1)])
+    free = torch.cat([t["free_pages"], t["free_pages"].new_zeros(1)])
     P = free.numel() - 1
     rr = rel.flatten().long().cumsum(0) - rel.flatten().long()
     dst = torch.where(rel.flatten() & ok, n_free + nrel - 1 - rr, torch.full_like(rr, P))
@@ -362,7 +363,7 @@ def _plan_pages(t, need, drop):
     tr = take.flatten().long().cumsum(0) - take.flatten().long()
     src = (top - 1 - tr).clamp(0, P - 1)
     new_bt = torch.where(take.flatten() & ok, free[src], bt.flatten()).view(B, mp)
-    t["free"].copy_(torch.where(ok, free, t["free"]))
+    t["free_pages"].copy_(torch.where(ok, free, t["free_pages"]))
     bt.copy_(new_bt)
     t["held"].copy_(torch.where(ok, torch.maximum(keep, need.long()), held))
     t["n_free"].copy_(torch.where(ok, top - ntake, n_free))
@@ -645,7 +646,7 @@ def _exact_plan(case, seed):
     rows(ctx, new)
     rs = np.concatenate([[0], np.cumsum(new)])
     ks = np.concatenate([[0], np.cumsum(np.where(new > 0, ctx + new, 0))])
-    res = dict(block_table=bt, held=held, free=full, n_free=np.array([len(stack)]), row_start=rs, kv_start=ks,
+    res = dict(block_table=bt, held=held, free_pages=full, n_free=np.array([len(stack)]), row_start=rs, kv_start=ks,
                slot=slot, pos=pos, row_seq=seq, status=np.zeros(1, np.int64))
     return {n: torch.tensor(res[n], device=DEV).int() for n in TABLES}
 
