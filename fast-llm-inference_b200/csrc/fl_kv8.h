@@ -1,0 +1,105 @@
+// Private to the 8-bit paged KV cache sources (kv8.cu, kv8_attn.cu): the
+// handle, the device tables of a plan and the layout of the codes.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <vector>
+
+#include "fl_cuda.h"
+#include "fl_kernels.h"
+
+namespace fl {
+
+constexpr int kKv8Block = FL_KV8_BLOCK;           // positions per scale
+constexpr int kKv8Sub = kPageSize / kKv8Block;    // scales per page and head
+
+// Codes of one (page, kv head) are kPageSize * head_dim bytes: per block of
+// 16 positions, per chunk of 32 dimensions, 512 bytes in the order in which a
+// warp's lanes feed them to mma.m16n8k16, 16 bytes a lane, so that a block
+// is read with one coalesced 16-byte load per lane and chunk, straight into
+// the registers that the products use:
+//   K, lane 4 n + t: 8 dimensions 8 t .. 8 t + 7 of the two positions
+//      4 (n >> 1) + (n & 1) and that + 2 (the columns n of the two 8-wide
+//      score tiles of the block)
+//   V, lane 4 c + t: the 4 dimensions 4 c .. 4 c + 3, each for the four
+//      positions 4 t .. 4 t + 3 (the probabilities that lane t of a row holds)
+// INT8 codes are stored offset by 128, so that byte u under 0x64 is the half
+// 1024 + u and the value is that less 1152, exact.
+__host__ __device__ __forceinline__ int kv8_k_off(int pos, int d) {
+    const int n = 2 * (pos >> 2) + (pos & 1), half = (pos >> 1) & 1;
+    return (d >> 5) * 512 + n * 64 + ((d & 31) >> 3) * 16 + half * 8 + (d & 7);
+}
+__host__ __device__ __forceinline__ int kv8_v_off(int pos, int d) {
+    return (d >> 5) * 512 + ((d & 31) >> 2) * 64 + (pos >> 2) * 16 + (d & 3) * 4 + (pos & 3);
+}
+
+// One work item of the attention: a tile of packed query rows of a sequence
+// (packed row p: token p / group, query head kv_head * group + p % group)
+// over a range of its pages.
+struct Kv8Item {
+    int seq, tile, page0, pages;
+    int split, splits;   // this range among the tile's; 1 = the whole context
+    int part;            // first partial slot of the tile (splits > 1)
+    int pad;
+};
+
+// Counts and constants that a plan leaves on the device.
+struct Kv8Meta {
+    int seqs, rows, units, gblocks, items, pad[3];
+};
+
+// Device arrays of a plan (all owned by the handle).
+struct Kv8Tables {
+    int *block_table, *held, *free_pages, *n_free, *row_start, *kv_start, *slot, *pos, *row_seq, *status;
+    int *ctx;          // [max_seqs] cached positions of the planned sequences
+    int *take_start, *rel_start, *unit_start, *gblk_start, *item_start, *part_start;  // [max_seqs + 1]
+    int *unit_row;     // [max_rows] first row of every (sequence, 16-position block) touched
+    Kv8Item* items;
+    Kv8Meta* meta;
+};
+
+}  // namespace fl
+
+struct fl_kv8 {
+    fl_kv8_config_t c;
+    int device = 0, sms = 148;
+    int max_pages = 0;          // pages per sequence
+    int group = 1, tile_rows = 16;
+    int items_cap = 0, parts_cap = 0, target = 0;
+    int max_new = 0;            // bound of the last plan
+    int nseq = 0;
+    std::vector<void*> bufs;
+    std::vector<uint8_t*> k, v;       // [layers] codes
+    std::vector<float*> ks, vs;       // [layers] scales
+    fl::Kv8Tables t = {};
+    float* part = nullptr;      // [parts][kv_heads][tile_rows][head_dim] partial outputs
+    float2* part_ml = nullptr;  // [parts][kv_heads][tile_rows] (maximum, sum)
+    int* part_cnt = nullptr;    // [parts][kv_heads] arrivals, zero between launches
+};
+
+namespace fl {
+
+struct Kv8AttnParams {
+    const uint8_t *k, *v;
+    const float *ks, *vs;
+    Kv8Tables t;
+    int max_pages, heads, kv_heads, group, head_dim, type, dtype;
+    const void* q;
+    void* out;
+    size_t ldq, ldo;
+    int rows;            // rows of q and out
+    float scale;         // of the scores, times log2(e)
+    const uint8_t* mask; // [rows][ldm] or null: causal
+    int ldm;
+    float* part;
+    float2* part_ml;
+    int* part_cnt;
+};
+cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int ctas, cudaStream_t s);
+// CTAs of the attention kernel that one SM holds (for the plan's split).
+int kv8_attention_occupancy(int head_dim, int type, int dtype);
+
+}  // namespace fl

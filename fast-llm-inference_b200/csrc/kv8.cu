@@ -1,0 +1,792 @@
+// Paged KV cache in 8 bits for ragged batches: the handle, the plan (block
+// tables, slot maps and work lists from request lengths), the append and the
+// gather. The rules are stated in include/fl_cuda.h.
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+
+#include "fl_common.cuh"
+#include "fl_kv8.h"
+#include "fl_kv8_types.cuh"
+#include "fl_runtime.h"
+
+namespace fl {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// Plan: one kernel of one thread-block cluster. CTA 0 checks the lengths and
+// scans them; after a cluster barrier all CTAs return and take pages and write
+// the rows' maps and the work lists. Bound by latency: a chain of the length
+// loads, the scans and the page loads, with barriers between; the row maps of
+// a prompt batch are what the other CTAs are there for.
+// ---------------------------------------------------------------------------
+constexpr int kPT = 1024;
+
+struct PlanArgs {
+    const int *ctx, *nw;
+    Kv8Tables t;
+    int nseq, max_new, max_pages, max_rows;
+    int group, tile_rows, kv_heads, target;
+};
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Exclusive prefix sum of one value per thread; the total to every thread.
+__device__ int block_scan(int v, int* red, int* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = inc;
+    __syncthreads();
+    int w = red[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+    }
+    *total = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    return (warp ? before : 0) + inc - v;
+}
+
+__device__ long long block_sum64(long long v, long long* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    long long t = red[threadIdx.x & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    return t;
+}
+
+struct SeqPlan {
+    int n, ctx, keep, need;   // new rows, cached positions, pages kept, pages held afterwards
+    int rel;                  // pages returned
+    bool bad;
+};
+
+__device__ __forceinline__ SeqPlan seq_plan(const PlanArgs& a, int b) {
+    SeqPlan s;
+    const int nw = a.nw[b], held = __ldcg(a.t.held + b);
+    s.bad = false;
+    s.n = max(nw, 0);
+    s.ctx = 0;
+    s.rel = nw < 0 ? held : 0;
+    s.keep = nw < 0 ? 0 : held;
+    s.need = s.keep;
+    if (s.n > 0) {
+        const int c = a.ctx[b];
+        const long long n = (long long)c + s.n;
+        s.bad = c < 0 || s.n > a.max_new || n > (long long)a.max_pages * kPageSize;
+        if (!s.bad) {
+            s.ctx = c;
+            s.need = max(s.keep, (int)((n + kPageSize - 1) / kPageSize));
+        }
+    }
+    return s;
+}
+
+// The first index b with start[b + 1] > r, start ascending, start[nseq] > r.
+__device__ __forceinline__ int find_seq(const int* start, int nseq, int r) {
+    int lo = 0, hi = nseq - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldcg(start + mid + 1) > r) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
+    __shared__ int red[32];
+    __shared__ long long red64[32];
+    uint32_t rank, nrank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
+    const Kv8Tables& t = a.t;
+    const int C = (a.nseq + kPT - 1) / kPT;
+    const int b0 = min(a.nseq, (int)threadIdx.x * C), b1 = min(a.nseq, b0 + C);
+    if (rank == 0) {
+        long long rows = 0, take = 0, rel = 0, bad = 0;
+        for (int b = b0; b < b1; b++) {
+            const SeqPlan s = seq_plan(a, b);
+            bad += s.bad;
+            rows += s.n;
+            take += s.need - s.keep;
+            rel += s.rel;
+        }
+        bad = block_sum64(bad, red64);
+        rows = block_sum64(rows, red64);
+        take = block_sum64(take, red64);
+        rel = block_sum64(rel, red64);
+        const long long have = (long long)__ldcg(t.n_free) + rel;
+        const int st = bad > 0 || rows > a.max_rows ? -1 : take > have ? (int)min(take - have, 0x7fffffffll) : 0;
+        if (threadIdx.x == 0) *t.status = st;
+        if (st != 0) {
+            for (int b = threadIdx.x; b <= a.nseq; b += kPT) t.row_start[b] = t.kv_start[b] = 0;
+            if (threadIdx.x == 0) *t.meta = Kv8Meta{a.nseq, 0, 0, 0, 0, {1, 0, 0}};
+        } else {
+            // sums of this thread's sequences, then the prefixes
+            int v[6] = {};
+            long long w = 0;   // (row tile, page) pairs: the attention's work
+            for (int b = b0; b < b1; b++) {
+                const SeqPlan s = seq_plan(a, b);
+                const int n = s.n ? s.ctx + s.n : 0;
+                v[0] += s.n;
+                v[1] += n;
+                v[2] += s.rel;
+                v[3] += s.need - s.keep;
+                v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
+                v[5] += (n + kKv8Block - 1) / kKv8Block;
+                w += (long long)((s.n * a.group + a.tile_rows - 1) / a.tile_rows) * ((n + kPageSize - 1) / kPageSize);
+            }
+            int tot[6];
+#pragma unroll
+            for (int i = 0; i < 6; i++) v[i] = block_scan(v[i], red, &tot[i]);
+            w = block_sum64(w, red64);
+            // pages per item: as few as make about `target` items over all heads
+            const long long want = max(1, a.target / a.kv_heads);
+            const int per = (int)max(1ll, (w + want - 1) / want);
+            int ni = 0, np = 0, toti, totp;
+            for (int b = b0; b < b1; b++) {
+                const SeqPlan s = seq_plan(a, b);
+                if (!s.n) continue;
+                const int tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
+                const int pages = (s.ctx + s.n + kPageSize - 1) / kPageSize, sp = (pages + per - 1) / per;
+                ni += tiles * sp;
+                np += sp > 1 ? tiles * sp : 0;
+            }
+            ni = block_scan(ni, red, &toti);
+            np = block_scan(np, red, &totp);
+            for (int b = b0; b < b1; b++) {
+                const SeqPlan s = seq_plan(a, b);
+                const int n = s.n ? s.ctx + s.n : 0;
+                t.ctx[b] = s.ctx;
+                t.row_start[b] = v[0];
+                t.kv_start[b] = v[1];
+                t.rel_start[b] = v[2];
+                t.take_start[b] = v[3];
+                t.unit_start[b] = v[4];
+                t.gblk_start[b] = v[5];
+                t.item_start[b] = ni;
+                t.part_start[b] = np;
+                v[0] += s.n;
+                v[1] += n;
+                v[2] += s.rel;
+                v[3] += s.need - s.keep;
+                v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
+                v[5] += (n + kKv8Block - 1) / kKv8Block;
+                if (s.n) {
+                    const int tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
+                    const int pages = (n + kPageSize - 1) / kPageSize, sp = (pages + per - 1) / per;
+                    ni += tiles * sp;
+                    np += sp > 1 ? tiles * sp : 0;
+                }
+            }
+            if (threadIdx.x == 0) {
+                t.row_start[a.nseq] = tot[0];
+                t.kv_start[a.nseq] = tot[1];
+                t.rel_start[a.nseq] = tot[2];
+                t.take_start[a.nseq] = tot[3];
+                t.unit_start[a.nseq] = tot[4];
+                t.gblk_start[a.nseq] = tot[5];
+                t.item_start[a.nseq] = toti;
+                t.part_start[a.nseq] = totp;
+                *t.meta = Kv8Meta{a.nseq, tot[0], tot[4], tot[5], toti, {0, per, 0}};
+            }
+        }
+    }
+    cluster_sync();
+    if (__ldcg(&t.meta->pad[0])) return;   // refused: nothing changes (every CTA alike)
+    const int per = __ldcg(&t.meta->pad[1]);
+    const int nfree = __ldcg(t.n_free), top = nfree + __ldcg(t.rel_start + a.nseq);
+    const int lane = threadIdx.x & 31;
+    const int wid = (int)rank * (kPT / 32) + (threadIdx.x >> 5), nw = (int)nrank * (kPT / 32);
+    // returned pages: the first page of the first sequence ends on top
+    for (int b = wid; b < a.nseq; b += nw)
+        if (a.nw[b] < 0) {
+            const int held = __ldcg(t.held + b), r0 = __ldcg(t.rel_start + b);
+            for (int j = lane; j < held; j += 32)
+                t.free_pages[top - 1 - r0 - j] = __ldcg(t.block_table + (size_t)b * a.max_pages + j);
+        }
+    cluster_sync();
+    // taken pages, and each sequence's shares of the work lists
+    for (int b = wid; b < a.nseq; b += nw) {
+        const SeqPlan s = seq_plan(a, b);
+        const int t0 = __ldcg(t.take_start + b);
+        for (int j = s.keep + lane; j < s.need; j += 32)
+            t.block_table[(size_t)b * a.max_pages + j] = __ldcg(t.free_pages + top - 1 - t0 - (j - s.keep));
+        __syncwarp();
+        if (lane == 0) t.held[b] = s.need;
+        if (!s.n) continue;
+        const int n = s.ctx + s.n;
+        const int r0 = __ldcg(t.row_start + b), u0 = __ldcg(t.unit_start + b);
+        const int units = (n - 1) / kKv8Block - s.ctx / kKv8Block + 1;
+        for (int u = lane; u < units; u += 32)
+            t.unit_row[u0 + u] = r0 + (u ? u * kKv8Block - s.ctx % kKv8Block : 0);
+        const int tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
+        const int pages = (n + kPageSize - 1) / kPageSize, sp = (pages + per - 1) / per;
+        const int i0 = __ldcg(t.item_start + b), p0 = __ldcg(t.part_start + b);
+        for (int i = lane; i < tiles * sp; i += 32) {
+            const int tile = i / sp, k = i - tile * sp;
+            // even shares: the first pages % sp ranges are one page longer
+            const int base = pages / sp, rem = pages - base * sp;
+            t.items[i0 + i] = Kv8Item{b, tile, k * base + min(k, rem), base + (k < rem ? 1 : 0),
+                                      k, sp, sp > 1 ? p0 + tile * sp : 0, 0};
+        }
+    }
+    cluster_sync();
+    if (rank == 0 && threadIdx.x == 0) *t.n_free = top - __ldcg(t.take_start + a.nseq);
+    const int rows = __ldcg(t.row_start + a.nseq);
+    for (int r = (int)rank * kPT + threadIdx.x; r < rows; r += (int)nrank * kPT) {
+        const int b = find_seq(t.row_start, a.nseq, r);
+        const int p = __ldcg(t.ctx + b) + r - __ldcg(t.row_start + b);
+        t.pos[r] = p;
+        t.row_seq[r] = b;
+        t.slot[r] = __ldcg(t.block_table + (size_t)b * a.max_pages + p / kPageSize) * kPageSize + p % kPageSize;
+    }
+}
+
+// Fresh tables: every page free (page 0 on top), nothing held.
+__global__ void kv8_reset_kernel(const Kv8Tables t, int pages, int max_seqs) {
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < pages; i += gridDim.x * blockDim.x)
+        t.free_pages[i] = pages - 1 - i;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < max_seqs; i += gridDim.x * blockDim.x) t.held[i] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        *t.n_free = pages;
+        *t.status = 0;
+        *t.meta = Kv8Meta{};
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Append: one warp per (16-position block touched, kv head, K or V). A lane
+// holds the 16 codes of its 16 stored bytes per chunk of 32 dimensions (see
+// fl_kv8.h), so the block's largest value is one warp reduction, and a stored
+// piece is read, recoded where the scale grew, filled in and written whole.
+// Bound by bytes: the rows once in, the codes once out.
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+    Kv8Tables t;
+    const void *k, *v;
+    size_t ldk, ldv;
+    uint8_t *kc, *vc;
+    float *ks, *vs;
+    int rows, kv_heads, vec;
+};
+
+constexpr int kAppendWarps = 8;
+
+// The lane's 16 values (or codes) of a chunk are four groups of four: group i
+// of a K piece is position i / 2's dimensions 4 (i & 1) .. + 3 (the bytes of
+// word i), of a V piece position i's four dimensions (byte i of every word).
+template <bool V>
+__device__ __forceinline__ int piece_pos(int lane, int i) {
+    const int n = lane >> 2, t = lane & 3;
+    return V ? 4 * t + i : 4 * (n >> 1) + (n & 1) + (i >> 1) * 2;
+}
+template <bool V>
+__device__ __forceinline__ int piece_dim(int lane, int i) {
+    return V ? (lane >> 2) * 4 : (lane & 3) * 8 + (i & 1) * 4;
+}
+template <bool V>
+__device__ __forceinline__ uint8_t piece_get(const uint32_t (&w)[4], int i, int j) {
+    return (uint8_t)(V ? w[j] >> (8 * i) : w[i] >> (8 * j));
+}
+template <bool V>
+__device__ __forceinline__ void piece_set(uint32_t (&w)[4], int i, int j, uint8_t c) {
+    uint32_t& x = V ? w[j] : w[i];
+    const int sh = 8 * (V ? i : j);
+    x = (x & ~(0xffu << sh)) | ((uint32_t)c << sh);
+}
+
+// Rows x[0 .. m) (row stride ld) into positions first .. first + m of a block.
+template <int HD, int DT, bool E4M3, bool V>
+__device__ __forceinline__ void append_block(const void* x, size_t at, size_t ld, int vec, int first, int m,
+                                             uint8_t* code, float* sp, int lane) {
+    constexpr int NC = HD / 32;
+    float val[NC][16];
+    float amax = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int p = piece_pos<V>(lane, i) - first;
+            float f[4] = {0.f, 0.f, 0.f, 0.f};
+            if (p >= 0 && p < m) load4<DT>(x, at + (size_t)p * ld + c * 32 + piece_dim<V>(lane, i), vec, f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                val[c][4 * i + j] = f[j];
+                const float y = fabsf(f[j]);
+                amax = fmaxf(amax, y < INFINITY ? y : 0.0f);   // NaN and infinities set no scale
+            }
+        }
+    float s = pow2_scale<E4M3>(warp_max(amax));
+    const float s_old = first > 0 ? *sp : s;
+    s = fmaxf(s, s_old);
+    const bool grew = s > s_old;
+    const float inv = pow2_inv(s), ratio = __fmul_rn(s_old, inv);
+    // a piece is written when it holds a new position, or an earlier one whose scale grew
+    bool fresh = false, old = false, gap = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int p = piece_pos<V>(lane, i) - first;
+        fresh |= p >= 0 && p < m;
+        old |= p < 0;
+        gap |= p < 0 || p >= m;
+    }
+    if (fresh || (grew && old)) {
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            uint4* pc = reinterpret_cast<uint4*>(code + c * 512);
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+            if (gap) {
+                const uint4 q = *pc;
+                w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int p = piece_pos<V>(lane, i) - first;
+                if (p >= 0 && p < m) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) piece_set<V>(w, i, j, encode8<E4M3>(__fmul_rn(val[c][4 * i + j], inv)));
+                } else if (p < 0 && grew) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        piece_set<V>(w, i, j, encode8<E4M3>(__fmul_rn(decode8<E4M3>(piece_get<V>(w, i, j)), ratio)));
+                }
+            }
+            *pc = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    __syncwarp();
+    if (lane == 0) *sp = s;
+}
+
+template <int HD, int DT, bool E4M3>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const AppendArgs a) {
+    const int lane = threadIdx.x & 31;
+    const Kv8Tables& t = a.t;
+    const int nrows = min(t.meta->rows, a.rows), units = t.meta->units;
+    const long long total = (long long)units * a.kv_heads * 2;
+    for (long long w = (long long)blockIdx.x * kAppendWarps + (threadIdx.x >> 5); w < total;
+         w += (long long)gridDim.x * kAppendWarps) {
+        const int h = (int)((w >> 1) % a.kv_heads), u = (int)((w >> 1) / a.kv_heads);
+        const int r0 = t.unit_row[u];
+        if (r0 >= nrows) continue;
+        const int b = t.row_seq[r0], slot0 = t.slot[r0];
+        const int first = slot0 % kKv8Block;            // first new position of the block
+        const int m = min(kKv8Block - first, min(t.row_start[b + 1], nrows) - r0);
+        const size_t ph = (size_t)(slot0 / kPageSize) * a.kv_heads + h;
+        const int blk = slot0 % kPageSize / kKv8Block;
+        const size_t off = ph * (kPageSize * HD) + (size_t)blk * (kKv8Block * HD) + lane * 16;
+        const size_t sc = ph * kKv8Sub + blk;
+        if (w & 1)
+            append_block<HD, DT, E4M3, true>(a.v, (size_t)r0 * a.ldv + (size_t)h * HD, a.ldv, a.vec, first, m,
+                                             a.vc + off, a.vs + sc, lane);
+        else
+            append_block<HD, DT, E4M3, false>(a.k, (size_t)r0 * a.ldk + (size_t)h * HD, a.ldk, a.vec, first, m,
+                                              a.kc + off, a.ks + sc, lane);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Gather: the values that the codes of every planned sequence stand for,
+// packed [key][kv head][head_dim]. One warp per (16-position block, kv head,
+// K or V); bound by the bytes written.
+// ---------------------------------------------------------------------------
+struct GatherArgs {
+    Kv8Tables t;
+    const uint8_t *kc, *vc;
+    const float *ks, *vs;
+    void *ko, *vo;
+    int keys, kv_heads, max_pages, vec;
+};
+
+template <int HD, int DT, bool E4M3, bool V>
+__device__ __forceinline__ void gather_block(const uint8_t* code, float s, void* out, size_t at, size_t ld, int vec,
+                                             int m, int lane) {
+#pragma unroll
+    for (int c = 0; c < HD / 32; c++) {
+        const uint4 q = *reinterpret_cast<const uint4*>(code + c * 512);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int p = piece_pos<V>(lane, i);
+            if (p >= m) continue;
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[j] = __fmul_rn(decode8<E4M3>(piece_get<V>(w, i, j)), s);
+            store4<DT>(out, at + (size_t)p * ld + c * 32 + piece_dim<V>(lane, i), vec, f);
+        }
+    }
+}
+
+template <int HD, int DT, bool E4M3>
+__global__ void __launch_bounds__(kAppendWarps * 32) kv8_gather_kernel(const GatherArgs a) {
+    const int lane = threadIdx.x & 31;
+    const Kv8Tables& t = a.t;
+    const int nseq = t.meta->seqs;
+    const size_t ld = (size_t)a.kv_heads * HD;
+    const long long total = (long long)t.meta->gblocks * a.kv_heads * 2;
+    for (long long w = (long long)blockIdx.x * kAppendWarps + (threadIdx.x >> 5); w < total;
+         w += (long long)gridDim.x * kAppendWarps) {
+        const int h = (int)((w >> 1) % a.kv_heads), g = (int)((w >> 1) / a.kv_heads);
+        const int b = find_seq(t.gblk_start, nseq, g);
+        const int blk = g - t.gblk_start[b];
+        const int k0 = t.kv_start[b] + blk * kKv8Block;
+        const int m = min(kKv8Block, min(t.kv_start[b + 1], a.keys) - k0);
+        if (m <= 0) continue;
+        const size_t ph = (size_t)t.block_table[(size_t)b * a.max_pages + blk / kKv8Sub] * a.kv_heads + h;
+        const size_t off = ph * (kPageSize * HD) + (size_t)(blk % kKv8Sub) * (kKv8Block * HD) + lane * 16;
+        const size_t sc = ph * kKv8Sub + blk % kKv8Sub;
+        const size_t at = (size_t)k0 * ld + (size_t)h * HD;
+        if (w & 1)
+            gather_block<HD, DT, E4M3, true>(a.vc + off, a.vs[sc], a.vo, at, ld, a.vec, m, lane);
+        else
+            gather_block<HD, DT, E4M3, false>(a.kc + off, a.ks[sc], a.ko, at, ld, a.vec, m, lane);
+    }
+}
+
+int elem_size(int dtype) { return dtype == FL_F32 ? 4 : 2; }
+
+// Calls f<HD, DT, E4M3>() for the handle's configuration.
+template <template <int, int, bool> class F, typename... A>
+cudaError_t dispatch(const fl_kv8_config_t& c, A... args) {
+#define FL_KV8_HD(HD)                                                                                   \
+    if (c.head_dim == HD) {                                                                             \
+        if (c.type == FL_KV8_E4M3) {                                                                    \
+            if (c.dtype == FL_F32) return F<HD, FL_F32, true>::run(args...);                            \
+            if (c.dtype == FL_F16) return F<HD, FL_F16, true>::run(args...);                            \
+            return F<HD, FL_BF16, true>::run(args...);                                                  \
+        }                                                                                               \
+        if (c.dtype == FL_F32) return F<HD, FL_F32, false>::run(args...);                               \
+        if (c.dtype == FL_F16) return F<HD, FL_F16, false>::run(args...);                               \
+        return F<HD, FL_BF16, false>::run(args...);                                                     \
+    }
+    FL_KV8_HD(32)
+    FL_KV8_HD(64)
+    FL_KV8_HD(96)
+    FL_KV8_HD(128)
+#undef FL_KV8_HD
+    return cudaErrorInvalidValue;
+}
+
+template <int HD, int DT, bool E4M3>
+struct RunAppend {
+    static cudaError_t run(const AppendArgs* a, int grid, cudaStream_t s) {
+        kv8_append_kernel<HD, DT, E4M3><<<grid, kAppendWarps * 32, 0, s>>>(*a);
+        return cudaGetLastError();
+    }
+};
+template <int HD, int DT, bool E4M3>
+struct RunGather {
+    static cudaError_t run(const GatherArgs* a, int grid, cudaStream_t s) {
+        kv8_gather_kernel<HD, DT, E4M3><<<grid, kAppendWarps * 32, 0, s>>>(*a);
+        return cudaGetLastError();
+    }
+};
+
+// Common checks of the calls on a handle.
+int check_handle(const fl_kv8* h, const char* what) {
+    if (!h) return set_error(FL_E_INVAL, std::string(what) + ": handle is NULL");
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != h->device) {
+        cudaGetLastError();
+        return set_error(FL_E_STATE, std::string(what) + ": the cache lives on another device than the current one");
+    }
+    return FL_OK;
+}
+
+int check_layer(const fl_kv8* h, int layer, const char* what) {
+    FL_CHECK(check_handle(h, what));
+    if (layer < 0 || layer >= h->c.layers) return set_error(FL_E_INVAL, std::string(what) + ": no such layer");
+    if (h->nseq == 0) return set_error(FL_E_STATE, std::string(what) + ": no plan yet (fl_kv8_plan)");
+    return FL_OK;
+}
+
+bool aligned(const void* p, size_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0; }
+
+template <typename T>
+int alloc(fl_kv8* h, T** p, size_t count, bool zero) {
+    void* q = nullptr;
+    const size_t bytes = std::max<size_t>(count * sizeof(T), 16);
+    FL_CHECK_CUDA(cudaMalloc(&q, bytes));
+    h->bufs.push_back(q);
+    if (zero) FL_CHECK_CUDA(cudaMemset(q, 0, bytes));
+    *p = (T*)q;
+    return FL_OK;
+}
+
+int create(fl_kv8* h) {
+    const fl_kv8_config_t& c = h->c;
+    h->max_pages = (c.max_ctx + kPageSize - 1) / kPageSize;
+    h->group = c.heads / c.kv_heads;
+    h->tile_rows = c.dtype == FL_F32 ? 8 : 16;
+    cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device);
+    h->target = h->sms * kv8_attention_occupancy(c.head_dim, c.type, c.dtype);
+    const size_t S = c.max_seqs, R = c.max_rows, kvb = (size_t)c.pages * c.kv_heads * kPageSize * c.head_dim;
+    h->k.resize(c.layers);
+    h->v.resize(c.layers);
+    h->ks.resize(c.layers);
+    h->vs.resize(c.layers);
+    for (int l = 0; l < c.layers; l++) {
+        FL_CHECK(alloc(h, &h->k[l], kvb, true));
+        FL_CHECK(alloc(h, &h->v[l], kvb, true));
+        FL_CHECK(alloc(h, &h->ks[l], (size_t)c.pages * c.kv_heads * kKv8Sub, true));
+        FL_CHECK(alloc(h, &h->vs[l], (size_t)c.pages * c.kv_heads * kKv8Sub, true));
+    }
+    Kv8Tables& t = h->t;
+    FL_CHECK(alloc(h, &t.block_table, S * h->max_pages, true));
+    FL_CHECK(alloc(h, &t.held, S, true));
+    FL_CHECK(alloc(h, &t.free_pages, c.pages, true));
+    FL_CHECK(alloc(h, &t.n_free, 1, true));
+    FL_CHECK(alloc(h, &t.status, 1, true));
+    FL_CHECK(alloc(h, &t.slot, R, true));
+    FL_CHECK(alloc(h, &t.pos, R, true));
+    FL_CHECK(alloc(h, &t.row_seq, R, true));
+    FL_CHECK(alloc(h, &t.unit_row, R, true));
+    for (int** p : {&t.row_start, &t.kv_start, &t.take_start, &t.rel_start, &t.unit_start, &t.gblk_start, &t.item_start,
+                    &t.part_start, &t.ctx})
+        FL_CHECK(alloc(h, p, S + 1, true));
+    // a plan makes at most target / kv_heads items beyond one a tile, and
+    // splits only tiles of more pages than an item takes: at most twice that
+    // many partial results
+    const size_t want = std::max(1, h->target / c.kv_heads);
+    const size_t tiles = (R * h->group + h->tile_rows - 1) / h->tile_rows + S;
+    h->items_cap = (int)(tiles + want);
+    h->parts_cap = (int)(2 * want);
+    FL_CHECK(alloc(h, &t.items, h->items_cap, false));
+    FL_CHECK(alloc(h, &t.meta, 1, true));
+    const size_t np = (size_t)h->parts_cap * c.kv_heads;
+    FL_CHECK(alloc(h, &h->part, np * h->tile_rows * c.head_dim, false));
+    FL_CHECK(alloc(h, &h->part_ml, np * h->tile_rows, false));
+    FL_CHECK(alloc(h, &h->part_cnt, np, true));
+    kv8_reset_kernel<<<64, 256>>>(t, c.pages, c.max_seqs);
+    FL_CHECK_CUDA(cudaGetLastError());
+    FL_CHECK_CUDA(cudaDeviceSynchronize());
+    return FL_OK;
+}
+
+}  // namespace
+
+}  // namespace fl
+
+using namespace fl;
+
+FL_API fl_kv8_t* fl_kv8_create(const fl_kv8_config_t* cfg, int device) {
+    if (!cfg) {
+        set_error(FL_E_INVAL, "kv8_create: config is NULL");
+        return nullptr;
+    }
+    const fl_kv8_config_t c = *cfg;
+    const char* bad = nullptr;
+    if (c.layers < 1 || c.heads < 1 || c.kv_heads < 1 || c.pages < 1 || c.max_seqs < 1 || c.max_rows < 1 || c.max_ctx < 1)
+        bad = "kv8_create: every size must be at least 1";
+    else if (c.heads % c.kv_heads)
+        bad = "kv8_create: heads must be a multiple of kv_heads";
+    else if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 96 && c.head_dim != 128)
+        bad = "kv8_create: head_dim must be 32, 64, 96 or 128";
+    else if (c.type != FL_KV8_INT8 && c.type != FL_KV8_E4M3)
+        bad = "kv8_create: type must be FL_KV8_INT8 or FL_KV8_E4M3";
+    else if (c.dtype != FL_F32 && c.dtype != FL_F16 && c.dtype != FL_BF16)
+        bad = "kv8_create: dtype must be FL_F32, FL_F16 or FL_BF16";
+    else if (c.layers > 4096 || c.heads > 4096 || c.max_seqs > 65536 || c.pages > (1 << 24) || c.max_rows > (1 << 24) ||
+             c.max_ctx > (1 << 28) || (long long)c.max_rows * (c.heads / c.kv_heads) > (1 << 28))
+        bad = "kv8_create: a size is beyond its limit (4096 layers or heads, 65536 sequences, 2^24 pages or rows, "
+              "2^28 positions)";
+    if (bad) {
+        set_error(FL_E_INVAL, bad);
+        return nullptr;
+    }
+    if (ensure_device() != FL_OK) return nullptr;
+    int prev = 0, n = 0;
+    if (cudaGetDevice(&prev) != cudaSuccess || cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n) {
+        cudaGetLastError();
+        set_error(FL_E_INVAL, "kv8_create: no such device");
+        return nullptr;
+    }
+    fl_kv8* h = new (std::nothrow) fl_kv8;
+    if (!h) {
+        set_error(FL_E_NOMEM, "kv8_create: host allocation");
+        return nullptr;
+    }
+    h->c = c;
+    h->device = device;
+    int rc = FL_E_NOMEM;
+    if (cudaSetDevice(device) == cudaSuccess) {
+        try {
+            rc = create(h);
+        } catch (...) {   // host allocation; no exception leaves a C entry
+            rc = set_error(FL_E_NOMEM, "kv8_create: host allocation");
+        }
+    }
+    if (rc != FL_OK) {
+        fl_kv8_destroy(h);
+        h = nullptr;
+    }
+    cudaSetDevice(prev);
+    return h;
+}
+
+FL_API void fl_kv8_destroy(fl_kv8_t* h) {
+    if (!h) return;
+    int prev = 0;
+    cudaGetDevice(&prev);
+    cudaSetDevice(h->device);
+    for (void* p : h->bufs) cudaFree(p);
+    cudaSetDevice(prev);
+    delete h;
+}
+
+FL_API int fl_kv8_tables(const fl_kv8_t* h, fl_kv8_tables_t* out) {
+    if (!h || !out) return set_error(FL_E_INVAL, "kv8_tables: NULL argument");
+    const Kv8Tables& t = h->t;
+    *out = fl_kv8_tables_t{t.block_table, t.held, t.free_pages, t.n_free, t.row_start, t.kv_start,
+                           t.slot, t.pos, t.row_seq, t.status, h->max_pages};
+    return FL_OK;
+}
+
+FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int nseq, int max_new, void* stream) {
+    FL_CHECK(check_handle(h, "kv8_plan"));
+    if (!ctx_len || !new_len) return set_error(FL_E_INVAL, "kv8_plan: NULL lengths");
+    if (nseq < 1 || nseq > h->c.max_seqs) return set_error(FL_E_INVAL, "kv8_plan: nseq must be 1 .. max_seqs");
+    if (max_new < 1) return set_error(FL_E_INVAL, "kv8_plan: max_new must be at least 1");
+    cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
+    PlanArgs a = {};
+    a.ctx = ctx_len;
+    a.nw = new_len;
+    a.t = h->t;
+    a.nseq = nseq;
+    a.max_new = std::min(max_new, h->c.max_rows);
+    a.max_pages = h->max_pages;
+    a.max_rows = h->c.max_rows;
+    a.group = h->group;
+    a.tile_rows = h->tile_rows;
+    a.kv_heads = h->c.kv_heads;
+    a.target = h->target;
+    // one CTA while its threads hold the rows; eight (a portable cluster) beyond
+    const long long rows = std::min<long long>((long long)nseq * a.max_new, h->c.max_rows);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = rows > 4 * kPT ? 8 : 1;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(at[0].val.clusterDim.x);
+    cfg.blockDim = dim3(kPT);
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    FL_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kv8_plan_kernel, a));
+    h->nseq = nseq;
+    h->max_new = a.max_new;
+    return FL_OK;
+}
+
+FL_API int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, int rows, size_t ldk, size_t ldv,
+                         void* stream) {
+    FL_CHECK(check_layer(h, layer, "kv8_append"));
+    if (rows < 0) return set_error(FL_E_INVAL, "kv8_append: rows is negative");
+    if (rows == 0) return FL_OK;
+    const size_t w = (size_t)h->c.kv_heads * h->c.head_dim;
+    if (!k || !v) return set_error(FL_E_INVAL, "kv8_append: NULL rows");
+    if (rows > 1 && (ldk < w || ldv < w)) return set_error(FL_E_INVAL, "kv8_append: a row stride is below kv_heads * head_dim");
+    const int es = elem_size(h->c.dtype);
+    if ((uintptr_t)k % es || (uintptr_t)v % es) return set_error(FL_E_INVAL, "kv8_append: rows are not aligned to their type");
+    cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
+    AppendArgs a = {};
+    a.t = h->t;
+    a.k = k;
+    a.v = v;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.kc = h->k[layer];
+    a.vc = h->v[layer];
+    a.ks = h->ks[layer];
+    a.vs = h->vs[layer];
+    a.rows = rows;
+    a.kv_heads = h->c.kv_heads;
+    a.vec = aligned(k, ldk, es) && aligned(v, ldv, es);
+    const long long units = std::min<long long>(rows, rows / kKv8Block + 2ll * h->nseq) * a.kv_heads * 2;
+    const int grid = (int)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, (long long)h->sms * 32);
+    FL_CHECK_CUDA((dispatch<RunAppend>(h->c, &a, grid, s)));
+    return FL_OK;
+}
+
+FL_API int fl_kv8_gather(fl_kv8_t* h, int layer, void* k, void* v, int keys, void* stream) {
+    FL_CHECK(check_layer(h, layer, "kv8_gather"));
+    if (keys < 0) return set_error(FL_E_INVAL, "kv8_gather: keys is negative");
+    if (keys == 0) return FL_OK;
+    if (!k || !v) return set_error(FL_E_INVAL, "kv8_gather: NULL outputs");
+    const int es = elem_size(h->c.dtype);
+    if ((uintptr_t)k % es || (uintptr_t)v % es) return set_error(FL_E_INVAL, "kv8_gather: outputs are not aligned to their type");
+    cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
+    GatherArgs a = {};
+    a.t = h->t;
+    a.kc = h->k[layer];
+    a.vc = h->v[layer];
+    a.ks = h->ks[layer];
+    a.vs = h->vs[layer];
+    a.ko = k;
+    a.vo = v;
+    a.keys = keys;
+    a.kv_heads = h->c.kv_heads;
+    a.max_pages = h->max_pages;
+    a.vec = aligned(k, 16, es) && aligned(v, 16, es);
+    const long long units = ((long long)keys / kKv8Block + h->nseq) * a.kv_heads * 2;
+    const int grid = (int)std::min<long long>((units + kAppendWarps - 1) / kAppendWarps, (long long)h->sms * 32);
+    FL_CHECK_CUDA((dispatch<RunGather>(h->c, &a, grid, s)));
+    return FL_OK;
+}
+
+FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo,
+                            float scale, const uint8_t* mask, int ldm, void* stream) {
+    FL_CHECK(check_layer(h, layer, "kv8_attention"));
+    if (rows < 0) return set_error(FL_E_INVAL, "kv8_attention: rows is negative");
+    if (rows == 0) return FL_OK;
+    const size_t w = (size_t)h->c.heads * h->c.head_dim;
+    if (!q || !out) return set_error(FL_E_INVAL, "kv8_attention: NULL rows");
+    if (rows > 1 && (ldq < w || ldo < w)) return set_error(FL_E_INVAL, "kv8_attention: a row stride is below heads * head_dim");
+    if (!(scale == scale) || scale - scale != 0.0f) return set_error(FL_E_INVAL, "kv8_attention: scale is not finite");
+    const int es = elem_size(h->c.dtype);
+    if ((uintptr_t)q % es || (uintptr_t)out % es)
+        return set_error(FL_E_INVAL, "kv8_attention: rows are not aligned to their type");
+    if (mask && ldm < h->max_new) return set_error(FL_E_INVAL, "kv8_attention: mask rows are shorter than max_new");
+    cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
+    Kv8AttnParams p = {};
+    p.k = h->k[layer];
+    p.v = h->v[layer];
+    p.ks = h->ks[layer];
+    p.vs = h->vs[layer];
+    p.t = h->t;
+    p.max_pages = h->max_pages;
+    p.heads = h->c.heads;
+    p.kv_heads = h->c.kv_heads;
+    p.group = h->group;
+    p.head_dim = h->c.head_dim;
+    p.type = h->c.type;
+    p.dtype = h->c.dtype;
+    p.q = q;
+    p.out = out;
+    p.ldq = ldq;
+    p.ldo = ldo;
+    p.rows = rows;
+    p.scale = scale * 1.4426950408889634f;
+    p.mask = mask;
+    p.ldm = ldm;
+    p.part = h->part;
+    p.part_ml = h->part_ml;
+    p.part_cnt = h->part_cnt;
+    FL_CHECK_CUDA(launch_kv8_attention(p, h->target, s));
+    return FL_OK;
+}

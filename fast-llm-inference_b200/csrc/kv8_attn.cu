@@ -1,0 +1,419 @@
+// Attention over the paged 8-bit KV cache (fl_kv8.h): query rows of a ragged
+// batch against their sequences' pages, softmax online, sm_100a.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = e^(scale q_i . k_j - m_i)
+//
+// over the visible positions j, m_i a running reference of the maximum. Codes
+// enter mma.m16n8k16 as halves (INT8 and E4M3 codes are exact there); a
+// block's power-of-two scales multiply its scores, and its probabilities,
+// exactly. Rows of 8 dimensions and of 4 positions lie in the cache in the
+// products' operand order, so a warp reads a block of 16 positions with one
+// 16-byte load per lane and 32 dimensions, straight into registers.
+//
+// Queries enter as halves too, each row shifted by a power of two so that its
+// largest value lies in [2^14, 2^15): exact for fp16 and bf16 rows down to
+// 2^-29 of the row's largest value. An f32 row enters as two halves (value and
+// remainder, 22 bits together): a tile then holds 8 rows, their remainders in
+// the tile's other 8 rows, so the second half costs no further product. The
+// probabilities of f32 rows are split the same way.
+#include <math.h>
+
+#include "fl_common.cuh"
+#include "fl_kv8.h"
+#include "fl_kv8_types.cuh"
+
+namespace fl {
+
+namespace {
+
+constexpr int kAW = 4;   // warps per CTA: one per 16-position block of a page
+constexpr float kShift = 7.0f;   // probabilities enter as 2^7 p: 2^-21 of the largest is a normal half
+constexpr float kSlack = 8.0f;   // the reference follows the maximum once it lags by 2^8
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four codes of a word as two half pairs.
+template <bool E4M3>
+__device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (E4M3) {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    } else {
+        const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
+// 8 values at dimensions d .. d + 7 of a query row.
+template <int DT>
+__device__ __forceinline__ void load8(const void* q, size_t i, int vec, float (&f)[8]) {
+    float a[4], b[4];
+    load4<DT>(q, i, vec, a);
+    load4<DT>(q, i + 4, vec, b);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        f[j] = a[j];
+        f[4 + j] = b[j];
+    }
+}
+
+// Shift of a row with largest magnitude a: a 2^sh in [2^14, 2^15); 0 for a
+// zero row and for one that is not finite (its results are NaN).
+__device__ __forceinline__ float row_shift(float a) {
+    const int x = (int)((__float_as_uint(a) >> 23) & 255u);
+    if (x == 0 || x == 255) return 1.0f;
+    return __uint_as_float((uint32_t)min(max(127 + 14 - (x - 127), 1), 253) << 23);
+}
+
+template <int HD, int DT, bool E4M3>
+__global__ void __launch_bounds__(kAW * 32) kv8_attention_kernel(const Kv8AttnParams p, const int vec) {
+    constexpr bool F32 = DT == FL_F32;
+    constexpr int TR = F32 ? 8 : 16;   // query rows per tile
+    constexpr int NC = HD / 32;
+    constexpr int RR = F32 ? 1 : 2;    // rows of a thread
+    __shared__ float o_s[kAW][TR][HD];
+    __shared__ float m_s[kAW][TR], l_s[kAW][TR];
+    __shared__ int last_s;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t4 = lane & 3;
+    const long long work = (long long)p.t.meta->items * p.kv_heads;
+    for (long long w = blockIdx.x; w < work; w += gridDim.x) {
+        const Kv8Item it = p.t.items[w / p.kv_heads];
+        const int h = (int)(w % p.kv_heads);
+        const int ctx = p.t.ctx[it.seq], row0 = p.t.row_start[it.seq];
+        const int nb = p.t.row_start[it.seq + 1] - row0;
+        const int np = min(TR, nb * p.group - it.tile * TR);       // packed rows of the tile
+        const int tok_last = (it.tile * TR + np - 1) / p.group;
+        const int kend = p.mask ? ctx + nb : ctx + tok_last + 1;   // positions any row may see
+        // this thread's rows: token, query head
+        int row[RR], tok[RR], head[RR];
+        bool live[RR];
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+            const int pr = it.tile * TR + g + 8 * r;
+            tok[r] = pr / p.group;
+            head[r] = h * p.group + pr - tok[r] * p.group;
+            row[r] = row0 + tok[r];
+            live[r] = g + 8 * r < np && row[r] < p.rows;
+        }
+        // queries, shifted, as operand fragments: k step s of chunk c holds
+        // dimensions 32 c + 8 t4 + 4 s .. + 3
+        uint32_t qa[NC][2][4];
+        float unshift[RR];
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+            float amax = 0.0f;
+            float f[NC][8];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[c][j] = 0.0f;
+                if (live[r]) load8<DT>(p.q, (size_t)row[r] * p.ldq + (size_t)head[r] * HD + c * 32 + t4 * 8, vec, f[c]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) amax = fabsf(f[c][j]) > amax || f[c][j] != f[c][j] ? fabsf(f[c][j]) : amax;
+            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const float sh = row_shift(amax);
+            unshift[r] = pow2_inv(sh) * p.scale;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    float y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) y[j] = f[c][4 * s + j] * sh;
+                    qa[c][s][r] = h2(y[0], y[1]);
+                    qa[c][s][2 + r] = h2(y[2], y[3]);
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) y[j] -= __half2float(__float2half_rn(y[j]));
+                        qa[c][s][1] = h2(y[0], y[1]);
+                        qa[c][s][3] = h2(y[2], y[3]);
+                    }
+                }
+        }
+        float m[RR], l[RR];
+        float o[NC][4][4];
+        float vref = 0.0f;   // scale of the accumulators: the largest V scale so far
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[c][j][i] = 0.0f;
+
+        const int* bt = p.t.block_table + (size_t)it.seq * p.max_pages + it.page0;
+        for (int i = 0; i < it.pages; i++) {
+            const int pos0 = (it.page0 + i) * kPageSize + warp * kKv8Block;
+            if (pos0 >= kend) break;
+            const size_t ph = (size_t)bt[i] * p.kv_heads + h;
+            const size_t off = ph * (kPageSize * HD) + warp * (kKv8Block * HD) + lane * 16;
+            uint4 kq[NC], vq[NC];
+#pragma unroll
+            for (int c = 0; c < NC; c++) kq[c] = ld_stream16(p.k + off + c * 512);
+#pragma unroll
+            for (int c = 0; c < NC; c++) vq[c] = ld_stream16(p.v + off + c * 512);
+            const float ks = p.ks[ph * kKv8Sub + warp], vs = p.vs[ph * kKv8Sub + warp];
+            // positions behind the sequence may hold anything: an E4M3 byte there may be a NaN
+            if (E4M3 && pos0 + kKv8Block > ctx + nb) {
+                const int lim = ctx + nb - pos0 - 4 * t4;   // of this lane's four V positions
+                const uint32_t keep = lim >= 4 ? 0xffffffffu : lim <= 0 ? 0u : (1u << (8 * lim)) - 1u;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    vq[c].x &= keep; vq[c].y &= keep; vq[c].z &= keep; vq[c].w &= keep;
+                }
+            }
+            float sa[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                uint32_t b0, b1;
+                codes_to_halves<E4M3>(kq[c].x, b0, b1);
+                mma16816(sa[0], qa[c][0], b0, b1);
+                codes_to_halves<E4M3>(kq[c].z, b0, b1);
+                mma16816(sa[1], qa[c][0], b0, b1);
+                codes_to_halves<E4M3>(kq[c].y, b0, b1);
+                mma16816(sa[0], qa[c][1], b0, b1);
+                codes_to_halves<E4M3>(kq[c].w, b0, b1);
+                mma16816(sa[1], qa[c][1], b0, b1);
+            }
+            // scores (base 2) of row r at positions pos0 + 4 t4 + 2 half + e
+            float s[RR][4];
+#pragma unroll
+            for (int r = 0; r < RR; r++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float* a = sa[e >> 1];
+                    const float raw = F32 ? a[e & 1] + a[2 + (e & 1)] : a[2 * r + (e & 1)];
+                    s[r][e] = raw * ks * unshift[r];
+                }
+            if (p.mask || pos0 + kKv8Block > ctx) {
+#pragma unroll
+                for (int r = 0; r < RR; r++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int j = pos0 + 4 * t4 + e - ctx;   // new row, negative: cached
+                        bool see = j <= tok[r];
+                        if (p.mask && j >= 0) see = j < nb && live[r] && p.mask[(size_t)row[r] * p.ldm + j] != 0;
+                        if (!see) s[r][e] = -INFINITY;
+                    }
+            }
+            // reference of the maximum, and of the V scale
+            float mx[RR];
+            bool move = vs > vref;
+#pragma unroll
+            for (int r = 0; r < RR; r++) {
+                mx[r] = fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3]));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                move |= mx[r] > m[r] + kSlack || (m[r] == -INFINITY && mx[r] > m[r]);
+            }
+            if (__any_sync(0xffffffffu, move)) {
+                const float vnew = fmaxf(vs, vref);
+                const float vr = vref * pow2_inv(vnew);
+                vref = vnew;
+#pragma unroll
+                for (int r = 0; r < RR; r++) {
+                    const float mn = fmaxf(m[r], mx[r]);
+                    const float al = m[r] == -INFINITY ? 0.0f : exp2f(m[r] - mn);
+                    m[r] = mn;
+                    l[r] *= al;
+                    const float f = al * vr;
+#pragma unroll
+                    for (int c = 0; c < NC; c++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            o[c][j][2 * r] *= f;
+                            o[c][j][2 * r + 1] *= f;
+                            if constexpr (F32) {
+                                o[c][j][2] *= f;
+                                o[c][j][3] *= f;
+                            }
+                        }
+                }
+            }
+            uint32_t pa[4];
+            const float vf = vs * pow2_inv(vref);
+#pragma unroll
+            for (int r = 0; r < RR; r++) {
+                const float mr = m[r] == -INFINITY ? 0.0f : m[r] - kShift;
+                float pr[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    pr[e] = exp2f(s[r][e] - mr);
+                    l[r] += pr[e];
+                    pr[e] *= vf;
+                }
+                pa[r] = h2(pr[0], pr[1]);
+                pa[2 + r] = h2(pr[2], pr[3]);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) pr[e] -= __half2float(__float2half_rn(pr[e]));
+                    pa[1] = h2(pr[0], pr[1]);
+                    pa[3] = h2(pr[2], pr[3]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const uint32_t vw[4] = {vq[c].x, vq[c].y, vq[c].z, vq[c].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t b0, b1;
+                    codes_to_halves<E4M3>(vw[j], b0, b1);
+                    mma16816(o[c][j], pa, b0, b1);
+                }
+            }
+        }
+        // this warp's result: reference, sum, normalised output
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RR; r++) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            const float f = l[r] != 0.0f ? __fdiv_rn(vref, l[r]) : 0.0f;   // NaN sums stay NaN
+            if (t4 == 0) {
+                m_s[warp][g + 8 * r] = m[r];
+                l_s[warp][g + 8 * r] = l[r];
+            }
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float4 v;
+                    float* vp = reinterpret_cast<float*>(&v);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        vp[j] = (F32 ? o[c][j][e] + o[c][j][2 + e] : o[c][j][2 * r + e]) * f;
+                    *reinterpret_cast<float4*>(&o_s[warp][g + 8 * r][c * 32 + 8 * t4 + 4 * e]) = v;
+                }
+        }
+        __syncthreads();
+        // joined over the warps: the weights are l 2^(m - M)
+        const size_t slot = (size_t)(it.part + it.split) * p.kv_heads + h;
+        for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kAW * 32) {
+            const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+            float M = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < kAW; k++) M = fmaxf(M, m_s[k][r]);
+            float L = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kAW; k++) {
+                if (l_s[k][r] == 0.0f) continue;
+                const float wk = l_s[k][r] * exp2f(m_s[k][r] - M);
+                L += wk;
+                const float4 v = *reinterpret_cast<const float4*>(&o_s[k][r][d]);
+                acc[0] += wk * v.x; acc[1] += wk * v.y; acc[2] += wk * v.z; acc[3] += wk * v.w;
+            }
+            const float f = L != 0.0f ? __fdiv_rn(1.0f, L) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[j] *= f;
+            if (it.splits > 1) {
+                *reinterpret_cast<float4*>(p.part + (slot * TR + r) * HD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                if (d == 0) p.part_ml[slot * TR + r] = make_float2(M, L);
+            } else {
+                const int pr = it.tile * TR + r, tk = pr / p.group;
+                const int hq = h * p.group + pr - tk * p.group;
+                if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
+            }
+        }
+        if (it.splits > 1) {
+            // the last range to arrive joins the tile's ranges, in their order
+            int* cnt = p.part_cnt + (size_t)it.part * p.kv_heads + h;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last_s = atomicAdd(cnt, 1) == it.splits - 1;
+            __syncthreads();
+            if (last_s) {
+                __threadfence();
+                const size_t s0 = (size_t)it.part * p.kv_heads + h;
+                for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kAW * 32) {
+                    const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+                    float M = -INFINITY;
+                    for (int k = 0; k < it.splits; k++)
+                        M = fmaxf(M, __ldcg(&p.part_ml[(s0 + (size_t)k * p.kv_heads) * TR + r]).x);
+                    float L = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int k = 0; k < it.splits; k++) {
+                        const size_t sk = (s0 + (size_t)k * p.kv_heads) * TR + r;
+                        const float2 ml = __ldcg(&p.part_ml[sk]);
+                        if (ml.y == 0.0f) continue;
+                        const float wk = ml.y * exp2f(ml.x - M);
+                        L += wk;
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + sk * HD + d));
+                        acc[0] += wk * v.x; acc[1] += wk * v.y; acc[2] += wk * v.z; acc[3] += wk * v.w;
+                    }
+                    const float f = L != 0.0f ? __fdiv_rn(1.0f, L) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[j] *= f;
+                    const int pr = it.tile * TR + r, tk = pr / p.group;
+                    const int hq = h * p.group + pr - tk * p.group;
+                    if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
+                }
+                if (threadIdx.x == 0) *cnt = 0;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Calls f with the kernel of a configuration.
+template <class F>
+cudaError_t with_kernel(int hd, int type, int dtype, F f) {
+#define FL_KV8_K(HD)                                                                                           \
+    if (hd == HD) {                                                                                            \
+        if (type == FL_KV8_E4M3)                                                                               \
+            return dtype == FL_F32   ? f(kv8_attention_kernel<HD, FL_F32, true>)                               \
+                   : dtype == FL_F16 ? f(kv8_attention_kernel<HD, FL_F16, true>)                               \
+                                     : f(kv8_attention_kernel<HD, FL_BF16, true>);                             \
+        return dtype == FL_F32   ? f(kv8_attention_kernel<HD, FL_F32, false>)                                  \
+               : dtype == FL_F16 ? f(kv8_attention_kernel<HD, FL_F16, false>)                                  \
+                                 : f(kv8_attention_kernel<HD, FL_BF16, false>);                                \
+    }
+    FL_KV8_K(32)
+    FL_KV8_K(64)
+    FL_KV8_K(96)
+    FL_KV8_K(128)
+#undef FL_KV8_K
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+int kv8_attention_occupancy(int head_dim, int type, int dtype) {
+    int n = 0;
+    with_kernel(head_dim, type, dtype, [&](auto* k) {
+        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kAW * 32, 0);
+    });
+    return n > 0 ? n : 1;
+}
+
+cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int ctas, cudaStream_t s) {
+    const int es = p.dtype == FL_F32 ? 4 : 2;
+    const int vec = ((uintptr_t)p.q & 15) == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldq * es % 16 == 0 &&
+                    p.ldo * es % 16 == 0;
+    return with_kernel(p.head_dim, p.type, p.dtype, [&](auto* k) {
+        k<<<ctas, kAW * 32, 0, s>>>(p, vec);
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace fl

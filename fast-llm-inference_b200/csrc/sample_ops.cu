@@ -23,6 +23,7 @@
 #include <limits.h>
 
 #include "fl_common.cuh"
+#include "fl_sample.cuh"
 #include "fl_state.h"
 
 namespace fl {
@@ -34,7 +35,6 @@ typedef unsigned __int128 u128;
 constexpr int kST = 1024;      // threads per row CTA
 constexpr int kSW = kST / 32;  // warps
 constexpr int kRegPT = 32;     // register-resident weights per thread
-constexpr uint32_t kOne = 1u << 24;
 
 __device__ uint32_t philox_u24(uint32_t seed, uint32_t seq, uint32_t step, uint32_t pos, uint32_t purpose) {
     uint32_t c0 = seq, c1 = step, c2 = pos, c3 = purpose;
@@ -51,25 +51,6 @@ __device__ uint32_t philox_u24(uint32_t seed, uint32_t seq, uint32_t step, uint3
         k1 += 0xBB67AE85u;
     }
     return c0 >> 8;
-}
-
-// E = trunc(e^x * 2^24) for x <= 0 (see the file comment).
-__device__ __forceinline__ uint32_t sample_weight(float x) {
-    if (!(x >= -17.0f)) return 0u;
-    const float kf = rintf(__fmul_rn(x, 1.442695f));
-    float r = __fmaf_rn(-kf, 0.693145751953125f, x);
-    r = __fmaf_rn(-kf, 1.4286068e-06f, r);
-    float p = 0.0001984127f;
-    p = __fmaf_rn(p, r, 0.0013888889f);
-    p = __fmaf_rn(p, r, 0.008333334f);
-    p = __fmaf_rn(p, r, 0.041666668f);
-    p = __fmaf_rn(p, r, 0.16666667f);
-    p = __fmaf_rn(p, r, 0.5f);
-    p = __fmaf_rn(p, r, 1.0f);
-    p = __fmaf_rn(p, r, 1.0f);
-    const int e = 127 + 24 + (int)kf;  // 2^(k + 24), k in [-25, 0]: a normal float
-    const uint32_t E = __float2uint_rz(__fmul_rn(p, __int_as_float(e << 23)));
-    return E > kOne ? kOne : E;
 }
 
 // Block-wide exact sum / float max; every thread gets the result.

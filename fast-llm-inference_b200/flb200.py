@@ -88,6 +88,18 @@ class DraftModel(C.Structure):
                 ("vocab_size", C.c_int)]
 
 
+class KV8Config(C.Structure):
+    """fl_kv8_config_t"""
+    _fields_ = [(n, C.c_int) for n in ("layers", "heads", "kv_heads", "head_dim", "pages", "max_seqs", "max_rows",
+                                       "max_ctx", "type", "dtype")]
+
+
+class KV8Tables(C.Structure):
+    """fl_kv8_tables_t"""
+    _fields_ = [(n, C.c_void_p) for n in ("block_table", "held", "free_pages", "n_free", "row_start", "kv_start", "slot",
+                                          "pos", "row_seq", "status")] + [("max_pages", C.c_int)]
+
+
 VP = C.c_void_p
 I = C.c_int
 F = C.c_float
@@ -121,6 +133,14 @@ _SIGS = {
     "fl_cuda_gemv_i8": (I, [VP, C.POINTER(DequantizedTensor), VP, I, I, I, VP]),
     "fl_cuda_block_dots_i8": (I, [VP, C.POINTER(DequantizedTensor), VP, I, I, I, VP]),
     "fl_cuda_block_dots_i8_noalloc": (I, [VP, C.POINTER(DequantizedTensor), VP, I, I, I, VP]),
+    "fl_kv8_create": (VP, [C.POINTER(KV8Config), I]),
+    "fl_kv8_destroy": (None, [VP]),
+    "fl_kv8_tables": (I, [VP, C.POINTER(KV8Tables)]),
+    "fl_kv8_plan": (I, [VP, VP, VP, I, I, VP]),
+    "fl_kv8_append": (I, [VP, I, VP, VP, I, SZ, SZ, VP]),
+    "fl_kv8_attention": (I, [VP, I, VP, VP, I, SZ, SZ, F, VP, I, VP]),
+    "fl_kv8_gather": (I, [VP, I, VP, VP, I, VP]),
+    "fl_cuda_sample": (I, [VP, I, SZ, I, I, VP, VP, VP, VP, VP, VP, VP]),
     "fl_synth_q4_0_i8": (I, [U64, U32, I, I, F, VP, VP]),
     "fl_synth_q4_0_i8_block": (I, [U64, U32, I, I, I, I, I, I, F, VP, VP]),
     "fl_synth_q4_0_f32": (I, [U64, U32, I, I, F, VP]),
@@ -301,6 +321,150 @@ def row_tensor(w: np.ndarray, s: np.ndarray) -> DequantizedTensor:
     t.scales_f16 = None
     t.dev = None
     return t
+
+
+# ------------------------------------------------- ragged batches, 8-bit KV cache
+# Arrays of these calls are device tensors with data_ptr(), dtype, shape,
+# stride() and device (torch tensors): the binding checks them and passes
+# their pointers. `stream` is a cudaStream_t as an integer (a torch stream's
+# cuda_stream; 0 is CUDA's default stream); None is the library's stream.
+DTYPES = {"float32": 0, "float16": 1, "bfloat16": 2}
+KV8_TYPES = {"int8": 0, "e4m3": 1}
+
+
+def _stream(stream):
+    return None if stream is None else stream or 1  # 1: cudaStreamLegacy
+
+
+def _dtype(t):
+    return str(t.dtype).rpartition(".")[2]
+
+
+def _device_array(t, name, dtype, shape, device):
+    """Pointer of a contiguous device tensor of this type and shape."""
+    if t.device.type != "cuda" or (device is not None and t.device.index != device):
+        raise FLError(f"{name} must be on cuda:{device}, not {t.device}")
+    if _dtype(t) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise FLError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, "
+                      f"not {_dtype(t)} {tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr()
+
+
+class _View:
+    """A device array of the library, for torch.as_tensor (no copy)."""
+
+    def __init__(self, ptr, shape, owner):
+        self.__cuda_array_interface__ = dict(shape=shape, typestr="<i4", data=(ptr, False), version=3, strides=None)
+        self._owner = owner
+
+
+class KV8Cache:
+    """Owns an fl_kv8_t: a paged KV cache in 8 bits and the plan of a ragged
+    batch's step (include/fl_cuda.h states the rules)."""
+
+    def __init__(self, lib: Lib, *, layers, heads, kv_heads, head_dim, pages, max_seqs, max_rows, max_ctx,
+                 type="int8", dtype="float32", device=0):
+        self.lib = lib
+        self.h = None
+        if type not in KV8_TYPES or dtype not in DTYPES:
+            raise FLError(f"type must be one of {list(KV8_TYPES)}, dtype one of {list(DTYPES)}")
+        self._c = KV8Config(layers, heads, kv_heads, head_dim, pages, max_seqs, max_rows, max_ctx, KV8_TYPES[type],
+                            DTYPES[dtype])
+        self.dtype, self.device = dtype, device
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        h = lib.fl_kv8_create(C.byref(self._c), device)
+        if not h:
+            raise FLError(f"fl_kv8_create failed: {lib.err()}")
+        self.h = h
+
+    def close(self):
+        if self.h:
+            self.lib.fl_kv8_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def tables(self):
+        """The plan's device arrays by name; views (torch.as_tensor shares
+        their memory) that keep the cache alive."""
+        t = KV8Tables()
+        self.lib.check(self.lib.fl_kv8_tables(self.h, C.byref(t)), "kv8_tables")
+        c = self._c
+        shapes = dict(block_table=(c.max_seqs, t.max_pages), held=(c.max_seqs,), free_pages=(c.pages,), n_free=(1,),
+                      row_start=(c.max_seqs + 1,), kv_start=(c.max_seqs + 1,), slot=(c.max_rows,), pos=(c.max_rows,),
+                      row_seq=(c.max_rows,), status=(1,))
+        return {n: _View(getattr(t, n), s, self) for n, s in shapes.items()}
+
+    def _rows(self, t, name, heads):
+        """(pointer, rows, row stride) of [rows, heads, head_dim] with whole rows."""
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise FLError(f"{name} must be on cuda:{self.device}, not {t.device}")
+        sh, st = t.shape, t.stride()
+        if _dtype(t) != self.dtype or len(sh) != 3 or sh[1] != heads or sh[2] != self.head_dim:
+            raise FLError(f"{name} must be {self.dtype} [rows, {heads}, {self.head_dim}], not {_dtype(t)} {tuple(sh)}")
+        if (st[2] != 1 or st[1] != self.head_dim and heads > 1) or (sh[0] > 1 and st[0] < heads * self.head_dim):
+            raise FLError(f"{name} must have whole rows (strides {tuple(st)})")
+        return t.data_ptr(), sh[0], st[0] if sh[0] > 1 else heads * self.head_dim
+
+    def plan(self, ctx_len, new_len, max_new, stream=None):
+        """ctx_len, new_len: int32 device tensors [sequences]; max_new bounds new_len."""
+        n = int(ctx_len.shape[0])
+        self.lib.check(self.lib.fl_kv8_plan(self.h, _device_array(ctx_len, "ctx_len", "int32", (n,), self.device),
+                                            _device_array(new_len, "new_len", "int32", (n,), self.device), n, max_new,
+                                            _stream(stream)), "kv8_plan")
+
+    def append(self, layer, k, v, stream=None):
+        """k, v: [rows, kv_heads, head_dim] of the planned rows."""
+        kp, rows, ldk = self._rows(k, "k", self.kv_heads)
+        vp, rv, ldv = self._rows(v, "v", self.kv_heads)
+        if rows != rv:
+            raise FLError(f"k has {rows} rows, v {rv}")
+        self.lib.check(self.lib.fl_kv8_append(self.h, layer, kp, vp, rows, ldk, ldv, _stream(stream)), "kv8_append")
+
+    def attention(self, layer, q, out, scale=None, mask=None, stream=None):
+        """q, out: [rows, heads, head_dim]; mask: uint8 [rows, >= max_new], the
+        new rows of its sequence that a row sees (None: causal)."""
+        qp, rows, ldq = self._rows(q, "q", self.heads)
+        op, ro, ldo = self._rows(out, "out", self.heads)
+        if rows != ro:
+            raise FLError(f"q has {rows} rows, out {ro}")
+        mp, ldm = None, 0
+        if mask is not None:
+            ldm = int(mask.shape[-1])
+            mp = _device_array(mask, "mask", "uint8", (rows, ldm), self.device)
+        if scale is None:
+            scale = self.head_dim ** -0.5
+        self.lib.check(self.lib.fl_kv8_attention(self.h, layer, qp, op, rows, ldq, ldo, scale, mp, ldm, _stream(stream)),
+                       "kv8_attention")
+
+    def gather(self, layer, k, v, stream=None):
+        """k, v: contiguous [keys, kv_heads, head_dim] outputs."""
+        n = int(k.shape[0])
+        shape = (n, self.kv_heads, self.head_dim)
+        self.lib.check(self.lib.fl_kv8_gather(self.h, layer, _device_array(k, "k", self.dtype, shape, self.device),
+                                              _device_array(v, "v", self.dtype, shape, self.device), n, _stream(stream)),
+                       "kv8_gather")
+
+
+def sample(lib: Lib, logits, u, tokens, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+    """tokens[r] drawn from logits [rows, V] (rows may be strided) by u [rows]
+    (fl_cuda_sample); parameters are device tensors [rows] or None."""
+    dt = _dtype(logits)
+    if dt not in DTYPES or len(logits.shape) != 2 or logits.device.type != "cuda":
+        raise FLError(f"logits must be a device tensor [rows, V] of {list(DTYPES)}, not {dt} {tuple(logits.shape)}")
+    rows, V = logits.shape
+    ld, inner = logits.stride()
+    if inner != 1 and V > 1 or rows > 1 and ld < V:
+        raise FLError(f"logits must have whole rows (strides {logits.stride()})")
+    dev = logits.device.index
+    arr = [None if t is None else _device_array(t, n, d, (rows,), dev)
+           for t, n, d in ((temperature, "temperature", "float32"), (top_k, "top_k", "int32"), (top_p, "top_p", "float32"),
+                           (min_p, "min_p", "float32"), (u, "u", "float32"), (tokens, "tokens", "int32"))]
+    lib.check(lib.fl_cuda_sample(logits.data_ptr(), DTYPES[dt], max(ld, V), rows, V, *arr, _stream(stream)), "sample")
 
 
 PHI3_MINI = dict(vocab_size=32064, hidden_size=3072, intermediate_size=8192, num_layers=32, num_heads=32,

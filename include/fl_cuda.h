@@ -136,6 +136,136 @@ int fl_cuda_block_dots_i8_noalloc(const float* A, const dequantized_tensor_t* B,
                                   int M, int N, int K, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* ragged batches over a paged KV cache in 8 bits                       */
+/* ------------------------------------------------------------------ */
+
+/* One step of a batch of requests of differing lengths, for callers with a
+ * scheduler of their own (no counterpart in the reference): plan (block tables
+ * and slot maps on the GPU from the request lengths), append (new K / V rows
+ * quantised into the cache), attention over it, then the projections
+ * (fl_cuda_matmul_i8) and fl_cuda_sample. Pages hold 64 positions.
+ *
+ * Codes and scales. Every 16 positions (from a multiple of 16) of a head have
+ * one scale for K and one for V, a power of two s = 2^e: the smallest, e >=
+ * -100, with max |x| <= top * s over the block's finite values; top is 127 (INT8,
+ * codes -127 .. 127) or 448 (E4M3). A code is x / s rounded to nearest even,
+ * beyond the largest code to it (infinities too); NaN gives 0. Appending to a
+ * part-filled block keeps max(old scale, the new rows' scale); when that grows,
+ * the earlier codes q become q * s_old / s rounded again. Every scaling is
+ * exact, so a code has been rounded once per growth and nowhere else: an INT8
+ * value is off by less than one step, s / 2 for its own rounding plus at most
+ * s / 4 + s / 8 + ... for the growths before. Appending the same rows again
+ * gives the same codes; appending at an earlier position (a rolled-back draft)
+ * keeps the scale that the discarded rows left, unless it starts the block.
+ *
+ * A handle belongs to one device and is used by one stream at a time: plan,
+ * append, attention and gather of a step are ordered by the caller's stream,
+ * and captured graphs of one handle must not run at the same time. The calls
+ * allocate nothing and can be captured; fl_kv8_plan re-reads the lengths at
+ * every replay. `stream` NULL is the library's stream; pass cudaStreamLegacy
+ * ((void*)1) for CUDA's default stream. FL_E_STATE when the current device is
+ * not the handle's. */
+#define FL_F32  0
+#define FL_F16  1
+#define FL_BF16 2
+#define FL_KV8_INT8 0
+#define FL_KV8_E4M3 1
+#define FL_KV8_BLOCK 16      /* positions per scale */
+
+typedef struct fl_kv8 fl_kv8_t;
+
+typedef struct {
+    int layers;      /* caches, all under one plan                         */
+    int heads;       /* query heads, a multiple of kv_heads                 */
+    int kv_heads;
+    int head_dim;    /* 32, 64, 96 or 128                                   */
+    int pages;       /* pages in the pool (of every layer)                  */
+    int max_seqs;    /* sequences of a plan                                 */
+    int max_rows;    /* new rows of a plan, over all sequences              */
+    int max_ctx;     /* positions of a sequence (rounded up to a page)      */
+    int type;        /* FL_KV8_INT8 or FL_KV8_E4M3                          */
+    int dtype;       /* of K, V, Q and outputs: FL_F32, FL_F16 or FL_BF16   */
+} fl_kv8_config_t;
+
+/* The plan's device arrays (read them on the plan's stream). */
+typedef struct {
+    int* block_table;  /* [max_seqs][max_pages] page of every 64 positions  */
+    int* held;         /* [max_seqs] pages held                             */
+    int* free_pages;   /* [pages] stack of free pages; n_free is its height */
+    int* n_free;       /* [1] */
+    int* row_start;    /* [max_seqs + 1] first new row of each sequence     */
+    int* kv_start;     /* [max_seqs + 1] first key of each in a gather      */
+    int* slot;         /* [max_rows] page * 64 + offset of a new row        */
+    int* pos;          /* [max_rows] its position                           */
+    int* row_seq;      /* [max_rows] its sequence                           */
+    int* status;       /* [1] 0; pages missing; -1 a length out of range    */
+    int max_pages;     /* pages of a block table row                        */
+} fl_kv8_tables_t;
+
+/* NULL on failure (fl_cuda_last_error). Allocates every buffer: 2 * layers *
+ * pages * kv_heads * 64 * head_dim bytes of codes, 1 / (4 head_dim) of that in
+ * scales, the tables and the attention's workspace. */
+fl_kv8_t* fl_kv8_create(const fl_kv8_config_t* cfg, int device);
+void fl_kv8_destroy(fl_kv8_t* h);
+int fl_kv8_tables(const fl_kv8_t* h, fl_kv8_tables_t* out);
+
+/* Plans a step: sequence b < nseq has ctx_len[b] cached positions and gets
+ * new_len[b] new rows (device arrays); the rows of all sequences follow one
+ * another. new_len 0: the sequence idles and keeps its pages; negative: it
+ * ends and returns them. max_new bounds new_len (host). Pages are taken from
+ * the top of the free stack in (sequence, position) order as far as the
+ * sequence does not hold them yet, after the pages of ended sequences went
+ * back, the first page of the first of them uppermost. When the pages do not
+ * suffice, or a length is out of range (ctx < 0, new > max_new, more positions
+ * than max_ctx, more rows than max_rows), nothing changes, status says so and
+ * the step has no rows: append, attention and gather then do nothing. Entries
+ * of slot, pos and row_seq behind the last row stay as they were. */
+int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int nseq, int max_new, void* stream);
+
+/* Quantises the planned rows of K and V (rows of kv_heads * head_dim values,
+ * ldk / ldv elements apart; keys already rotated) into their slots. `rows` is
+ * what k and v hold: planned rows behind it are not read. */
+int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, int rows, size_t ldk, size_t ldv,
+                  void* stream);
+
+/* out = softmax(scale * q K^T) V for every planned row and query head (rows
+ * ldq / ldo elements apart), over its sequence's positions: the cached ones
+ * and, of the new ones, those at or before the row's (mask NULL) or those that
+ * mask[row * ldm + j] names for the sequence's j-th new row (ldm >= max_new).
+ * A row that sees nothing gives zeros. Rows behind the last planned one, and
+ * behind `rows`, are left as they were. Products are taken with halves and
+ * summed in 32 bits; f32 queries and their probabilities keep 22 bits. */
+int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo, float scale,
+                     const uint8_t* mask, int ldm, void* stream);
+
+/* The values that the codes of every planned sequence with new rows stand for,
+ * its cached and new positions in order, sequences one after another (kv_start):
+ * k and v [keys][kv_heads][head_dim]. Keys behind `keys` are not written. For
+ * moving sequences out of the cache. */
+int fl_kv8_gather(fl_kv8_t* h, int layer, void* k, void* v, int keys, void* stream);
+
+/* One token per logits row [rows][V] (ld elements apart, dtype FL_F32, FL_F16
+ * or FL_BF16, V <= 2^20) from the uniform numbers u[rows] in [0, 1), by the
+ * integer-weight rule of the sampled decoding (speculative.h), extended by
+ * top-k and min-p. All arrays are on the device; each parameter array [rows]
+ * may be NULL (off, temperature 1). For row r, with weights E_i =
+ * trunc(e^((l_i - max l) / T) 2^24), 0 below an exponent of -17:
+ *   temperature <= 0 (or NaN): the largest logit, the lowest index of equals;
+ *   top_k >= 1: the other tokens than the top_k largest logits get weight 0
+ *     (equal logits in index order);
+ *   top_p < 1: kept are the E_i >= t, t the largest integer whose kept mass
+ *     is at least max(1, trunc(top_p 2^24)) / 2^24 of all that is left;
+ *   min_p > 0: kept are the E_i >= trunc(min_p 2^24);
+ *   the token is the first whose running kept weight exceeds
+ *     trunc(trunc(u 2^24) total / 2^24).
+ * Sums are exact, so the token does not depend on how the work is divided.
+ * A NaN logit counts as -inf, +inf as the largest float; a row with nothing
+ * above -inf gives -1. */
+int fl_cuda_sample(const void* logits, int dtype, size_t ld, int rows, int V, const float* temperature,
+                   const int* top_k, const float* top_p, const float* min_p, const float* u, int* tokens,
+                   void* stream);
+
+/* ------------------------------------------------------------------ */
 /* seeded synthetic weights (the loader side; host code)               */
 /* ------------------------------------------------------------------ */
 
