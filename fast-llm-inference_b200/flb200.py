@@ -336,15 +336,21 @@ def _stream(stream):
     return None if stream is None else stream or 1  # 1: cudaStreamLegacy
 
 
+_names = {}  # dtype object -> name
+
+
 def _dtype(t):
-    return str(t.dtype).rpartition(".")[2]
+    n = _names.get(t.dtype)
+    if n is None:
+        n = _names[t.dtype] = str(t.dtype).rpartition(".")[2]
+    return n
 
 
 def _device_array(t, name, dtype, shape, device):
     """Pointer of a contiguous device tensor of this type and shape."""
-    if t.device.type != "cuda" or (device is not None and t.device.index != device):
+    if t.get_device() != device:
         raise FLError(f"{name} must be on cuda:{device}, not {t.device}")
-    if _dtype(t) != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if _dtype(t) != dtype or t.shape != shape or not t.is_contiguous():
         raise FLError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, "
                       f"not {_dtype(t)} {tuple(t.shape)} with strides {t.stride()}")
     return t.data_ptr()
@@ -401,7 +407,7 @@ class KV8Cache:
 
     def _rows(self, t, name, heads):
         """(pointer, rows, row stride) of [rows, heads, head_dim] with whole rows."""
-        if t.device.type != "cuda" or t.device.index != self.device:
+        if t.get_device() != self.device:
             raise FLError(f"{name} must be on cuda:{self.device}, not {t.device}")
         sh, st = t.shape, t.stride()
         if _dtype(t) != self.dtype or len(sh) != 3 or sh[1] != heads or sh[2] != self.head_dim:
@@ -454,13 +460,13 @@ def sample(lib: Lib, logits, u, tokens, temperature=None, top_k=None, top_p=None
     """tokens[r] drawn from logits [rows, V] (rows may be strided) by u [rows]
     (fl_cuda_sample); parameters are device tensors [rows] or None."""
     dt = _dtype(logits)
-    if dt not in DTYPES or len(logits.shape) != 2 or logits.device.type != "cuda":
+    dev = logits.get_device()
+    if dt not in DTYPES or len(logits.shape) != 2 or dev < 0:
         raise FLError(f"logits must be a device tensor [rows, V] of {list(DTYPES)}, not {dt} {tuple(logits.shape)}")
     rows, V = logits.shape
     ld, inner = logits.stride()
     if inner != 1 and V > 1 or rows > 1 and ld < V:
         raise FLError(f"logits must have whole rows (strides {logits.stride()})")
-    dev = logits.device.index
     arr = [None if t is None else _device_array(t, n, d, (rows,), dev)
            for t, n, d in ((temperature, "temperature", "float32"), (top_k, "top_k", "int32"), (top_p, "top_p", "float32"),
                            (min_p, "min_p", "float32"), (u, "u", "float32"), (tokens, "tokens", "int32"))]

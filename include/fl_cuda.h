@@ -245,7 +245,7 @@ int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows,
 int fl_kv8_gather(fl_kv8_t* h, int layer, void* k, void* v, int keys, void* stream);
 
 /* One token per logits row [rows][V] (ld elements apart, dtype FL_F32, FL_F16
- * or FL_BF16, V <= 2^20) from the uniform numbers u[rows] in [0, 1), by the
+ * or FL_BF16, V <= 262000) from the uniform numbers u[rows] in [0, 1), by the
  * integer-weight rule of the sampled decoding (speculative.h), extended by
  * top-k and min-p. All arrays are on the device; each parameter array [rows]
  * may be NULL (off, temperature 1). For row r, with weights E_i =
