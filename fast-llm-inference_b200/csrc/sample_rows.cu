@@ -5,15 +5,16 @@
 // include/fl_cuda.h.
 //
 // A row is held by one CTA, or by a cluster of up to eight: every thread reads
-// 32 tokens at most, once, turns them into weights and keeps those in
+// 64 tokens at most, once, turns them into weights and keeps those in
 // registers. A threshold (of top-k by count, of top-p by mass) is found by
-// bisection between weights lo and hi, at their geometric mean while they lie
-// apart: after a few passes over the registers the undecided weights fit a
-// list in shared memory, and the remaining passes touch one or two of them per
-// thread. Counts and masses share one 64-bit word (44 bits of mass, V < 2^20),
-// and a pass costs one barrier. The draw is a two-level prefix sum in token
-// order: warps' sums, then the lanes of the warp that the target falls into.
-// Bound by instructions: about 25 a token for its weight, 3 for each pass.
+// bisection between weights lo and hi, near their geometric mean: passes over
+// the registers until 128 weights are undecided, and those are compared all
+// with all at once. Counts and masses share one 64-bit word (44 bits of mass).
+// The draw is a prefix sum in token order: over the warps, each of which holds
+// a contiguous piece of the row, then within the one the target falls into.
+// Bound by instructions: about 25 a token for its weight, 3 for each of about
+// eight passes; few warps with much work each, because what a pass costs apart
+// from that are the warps' reductions.
 #include <float.h>
 #include <limits.h>
 
@@ -31,8 +32,14 @@ namespace {
 
 typedef unsigned __int128 u128;
 typedef unsigned long long u64;
-constexpr int kTok = 32;          // tokens per thread
-constexpr int kList = 2048;       // undecided weights of a CTA in shared memory
+constexpr int kTok = 64;          // tokens per thread
+constexpr int kPairs = 128;       // undecided weights compared all with all
+// In a register a weight carries a count of one above its 24 bits (and the
+// value 2^24): eight of them add up in one word, count and mass at once.
+constexpr uint32_t kTag = 1u << 28;
+#ifndef SAMPLE_FEW
+#define SAMPLE_FEW 2
+#endif
 constexpr int kMassBits = 44;
 constexpr u64 kMass = (1ull << kMassBits) - 1;
 
@@ -45,17 +52,17 @@ struct SampleArgs {
     int* tokens;
 };
 
-// A logit as the rule reads it: NaN counts as -inf, +inf as the largest float, -0 as 0.
-__device__ __forceinline__ float canon(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX) + 0.0f; }
+// A logit as the rule reads it: NaN counts as -inf, +inf as the largest float.
+__device__ __forceinline__ float canon(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 template <int DT>
 __device__ __forceinline__ float logit(const void* l, int i) {
     if constexpr (DT == FL_F32) return canon(static_cast<const float*>(l)[i]);
     else if constexpr (DT == FL_F16) return canon(__half2float(static_cast<const __half*>(l)[i]));
     else return canon(__bfloat162float(static_cast<const __nv_bfloat16*>(l)[i]));
 }
-// Orders floats as unsigned integers.
+// Orders floats as unsigned integers, -0 as 0.
 __device__ __forceinline__ uint32_t sortable(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float unsortable(uint32_t k) {
@@ -66,30 +73,49 @@ __device__ __forceinline__ uint32_t fixed24(float p) {
     return __float2uint_rz(__fmul_rn(fminf(fmaxf(p, 0.0f), 1.0f), 16777216.0f));
 }
 
-// Sum over the warp modulo 2^64, from three integer reductions of the word's parts.
-__device__ __forceinline__ u64 warp_sum64(u64 v) {
-    const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0xffffffu);
-    const uint32_t b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 24) & 0xffffffu);
-    const uint32_t c = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 48));
-    return (u64)a + ((u64)b << 24) + ((u64)c << 48);
+// Hides that x is what it was, so that a loop over the registers that uses it
+// is computed again where it stands: kept for later, its 64 results would
+// push the weights out of the registers.
+__device__ __forceinline__ void again(uint32_t& x) { asm volatile("" : "+r"(x)); }
+
+// sum += w where w >= t. The add is a multiply-add by a one that the compiler
+// does not see: it runs beside the comparison in the other pipe, which an add
+// would share (a pass over the registers took 40 % less).
+__device__ __forceinline__ void add_if_ge(uint32_t& sum, uint32_t w, uint32_t t, uint32_t one) {
+    asm("{\n\t.reg .pred p;\n\tsetp.ge.u32 p, %1, %2;\n\t@p mad.lo.u32 %0, %1, %3, %0;\n\t}"
+        : "+r"(sum)
+        : "r"(w), "r"(t), "r"(one));
+}
+
+// A count in the upper 20 bits and a mass in the lower 44 of a word.
+__device__ __forceinline__ u64 pack(u64 count, u64 mass) { return (count << kMassBits) + mass; }
+
+// Sum over the warp of at most 64 weights a lane (c of them, together m < 2^31), packed.
+__device__ __forceinline__ u64 warp_pack(uint32_t c, uint32_t m) {
+    const uint32_t a = __reduce_add_sync(0xffffffffu, m & 0xfffffu);
+    const uint32_t b = __reduce_add_sync(0xffffffffu, (m >> 20) | c << 16);
+    return pack(b >> 16, ((u64)(b & 0xffffu) << 20) + a);
 }
 
 // Reductions and prefix sums over the threads of a row's CTA or cluster.
 template <int NT, int CL>
 struct Row {
-    static constexpr int NW = NT / 32;
+    static constexpr int NW = NT / 32, NS = CL * NW, cl = CL;
     struct Shared {
-        u64 slot[2][CL * NW];
-        u64 cell[kTok * NW];
-        uint32_t list[kList];
-        int nlist, found;
+        u64 slot[2][NS];
+        uint32_t pairs[kPairs];
+        uint32_t own[CL > 1 ? kPairs : 1];   // this CTA's part of them
+        int n;
     };
     Shared& sm;
-    int lane, warp, rank;
+    int lane, warp, rank, me;   // me: this warp among all of the row
     int phase = 0;
+    uint32_t one = 1u;
 
     __device__ Row(Shared& s) : sm(s), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), rank(0) {
         if (CL > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        me = rank * NW + warp;
+        asm volatile("" : "+r"(one));
     }
     __device__ __forceinline__ void sync() {
         if constexpr (CL > 1)
@@ -97,52 +123,70 @@ struct Row {
         else
             __syncthreads();
     }
-    // lane 0 of every warp: v into this warp's slot of every CTA of the cluster
-    __device__ __forceinline__ void push(u64 v) {
-        u64* p = &sm.slot[phase][rank * NW + warp];
+    // Every warp's v (the same in its lanes) to all threads: read slots() after
+    // it. Two sets of slots in turn: a warp that is a pass ahead writes the other.
+    __device__ __forceinline__ const u64* share(u64 v) {
+        u64* p = &sm.slot[phase][me];
         if constexpr (CL > 1) {
-            const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
             if (lane < CL) {
                 uint32_t ra;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(lane));
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                             : "=r"(ra)
+                             : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(lane));
                 asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(ra), "l"(v) : "memory");
             }
         } else if (lane == 0) {
             *p = v;
         }
-    }
-    // Two slot sets in turn: a thread that is a pass ahead writes the other one.
-    __device__ __forceinline__ u64 sum(u64 v) {
-        push(warp_sum64(v));
         sync();
+        const u64* s = sm.slot[phase];
+        phase ^= 1;
+        return s;
+    }
+    __device__ __forceinline__ u64 sum(uint32_t c, uint32_t m) {
+        const u64* s = share(warp_pack(c, m));
         u64 t = 0;
 #pragma unroll
-        for (int i = 0; i < CL * NW; i += 32)
-            if (i + lane < CL * NW) t += sm.slot[phase][i + lane];
-        phase ^= 1;
-        return warp_sum64(t);
+        for (int i = 0; i < NS; i++) t += s[i];
+        return t;
     }
     __device__ __forceinline__ uint32_t max32(uint32_t v) {
-        push(__reduce_max_sync(0xffffffffu, v));
-        sync();
-        u64 t = 0;
+        const u64* s = share(__reduce_max_sync(0xffffffffu, v));
+        uint32_t t = 0;
 #pragma unroll
-        for (int i = 0; i < CL * NW; i += 32)
-            if (i + lane < CL * NW) t = max(t, sm.slot[phase][i + lane]);
-        phase ^= 1;
-        return __reduce_max_sync(0xffffffffu, (uint32_t)t);
+        for (int i = 0; i < NS; i++) t = max(t, (uint32_t)s[i]);
+        return t;
+    }
+    // v to the same place in every CTA of the cluster
+    __device__ __forceinline__ void store_all(uint32_t* p, uint32_t v) {
+        if constexpr (CL > 1) {
+            const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+#pragma unroll
+            for (int i = 0; i < CL; i++) {
+                uint32_t ra;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(i));
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(ra), "r"(v) : "memory");
+            }
+        } else {
+            *p = v;
+        }
     }
 };
 
-// (count, mass) of the weights at or above t among the thread's registers.
-__device__ __forceinline__ u64 at_least(const uint32_t (&w)[kTok], uint32_t t) {
-    uint32_t m = 0, c = 0;   // 32 weights of at most 2^24 sum below 2^30
+// Sum of the row's weights at or above t.
+template <class R>
+__device__ __forceinline__ u64 at_least(R& row, const uint32_t (&w)[kTok], uint32_t t) {
+    const uint32_t tt = t + kTag;
+    uint32_t m = 0, c = 0;   // 64 weights of at most 2^24 sum to 2^30 at most
 #pragma unroll
-    for (int i = 0; i < kTok; i++) {
-        m += w[i] >= t ? w[i] : 0u;
-        c += w[i] >= t;
+    for (int i = 0; i < kTok; i += 8) {
+        uint32_t g = 0;
+#pragma unroll
+        for (int j = i; j < i + 8; j++) add_if_ge(g, w[j], tt, row.one);
+        c += g >> 28;
+        m += g & (kTag - 1u);
     }
-    return ((u64)c << kMassBits) + m;
+    return row.sum(c, m);
 }
 
 // The largest t in [lo, hi) with ok(sum of the weights >= t), given that
@@ -151,52 +195,62 @@ __device__ __forceinline__ u64 at_least(const uint32_t (&w)[kTok], uint32_t t) {
 template <class R, class Ok>
 __device__ __forceinline__ uint32_t bisect(R& row, const uint32_t (&w)[kTok], uint32_t lo, uint32_t hi, u64& slo,
                                            u64& shi, Ok ok) {
-    auto middle = [&]() -> uint32_t {
-        if (hi >> 1 > lo) {
-            const uint32_t g = __float2uint_rz(sqrtf(__uint2float_rz(lo)) * sqrtf(__uint2float_rz(hi)));
-            return min(max(g, lo + 1), hi - 1);
-        }
-        return lo + (hi - lo) / 2u;
-    };
-    while (hi - lo > 1u && ((slo - shi) >> kMassBits) > kList) {
-        const uint32_t mid = middle();
-        const u64 s = row.sum(at_least(w, mid));
+    while (hi - lo > 1u && (slo - shi) >> kMassBits > kPairs) {
+        // the mean of their logarithms, roughly (of their float patterns)
+        const uint32_t b = (__float_as_uint(__uint2float_rz(lo)) + __float_as_uint(__uint2float_rz(hi))) / 2u;
+        const uint32_t mid = min(max(__float2uint_rz(__uint_as_float(b)), lo + 1u), hi - 1u);
+        const u64 s = at_least(row, w, mid);
         if (ok(s)) { lo = mid; slo = s; } else { hi = mid; shi = s; }
     }
     if (hi - lo <= 1u) return lo;
-    // the undecided weights of this CTA as a list
-    if (threadIdx.x == 0) row.sm.nlist = 0;
+    // the undecided weights of the whole row in every CTA, each against all of
+    // them: the threshold is the largest at which ok holds
+    for (int i = threadIdx.x; i < kPairs; i += R::NW * 32) row.sm.pairs[i] = 0u;
+    if (threadIdx.x == 0) row.sm.n = 0;
     __syncthreads();
+    uint32_t* list = row.cl > 1 ? row.sm.own : row.sm.pairs;
+    const uint32_t from = lo + kTag, span = hi - lo;
 #pragma unroll
-    for (int i = 0; i < kTok; i++)
-        if (w[i] >= lo && w[i] < hi) row.sm.list[atomicAdd(&row.sm.nlist, 1)] = w[i];
+    for (int i = 0; i < kTok; i++)   // in any order: their sums are exact
+        if (w[i] - from < span) list[atomicAdd(&row.sm.n, 1)] = w[i] - kTag;
     __syncthreads();
-    constexpr int PT = (kList + R::NW * 32 - 1) / (R::NW * 32);
-    const int n = row.sm.nlist;
-    uint32_t q[PT];
+    if constexpr (R::cl > 1) {
+        const int n = row.sm.n;
+        const u64* s = row.share(row.warp == 0 ? n : 0);
+        int at = 0;
 #pragma unroll
-    for (int i = 0; i < PT; i++) {
-        const int at = threadIdx.x + i * R::NW * 32;
-        q[i] = at < n ? row.sm.list[at] : 0u;
+        for (int i = 0; i < R::NS; i++) at += i < row.me - row.warp ? (int)s[i] : 0;
+        if (threadIdx.x < n) row.store_all(&row.sm.pairs[at + threadIdx.x], row.sm.own[threadIdx.x]);
+        row.sync();
     }
-    const u64 base = shi;
-    while (hi - lo > 1u) {
-        const uint32_t mid = middle();
-        uint32_t m = 0, c = 0;
-#pragma unroll
-        for (int i = 0; i < PT; i++) {
-            const bool in = q[i] >= mid;
-            m += in ? q[i] : 0u;
+    constexpr int TP = R::NW * 32 / kPairs;   // threads per weight
+    const uint32_t mine = row.sm.pairs[threadIdx.x / TP];
+    auto sums = [&](uint32_t t, bool strictly) -> u64 {   // of the pairs, by the TP threads of a weight
+        uint32_t c = 0, m = 0;   // 128 weights below 2^24, or equal to it: 2^31 at most
+#pragma unroll 8
+        for (int i = threadIdx.x % TP; i < kPairs; i += TP) {
+            const uint32_t f = row.sm.pairs[i];
+            const bool in = strictly ? f > t : f >= t;
+            m += in ? f : 0u;
             c += in;
         }
-        const u64 s = base + row.sum(((u64)c << kMassBits) + m);
-        if (ok(s)) { lo = mid; slo = s; } else { hi = mid; shi = s; }
-    }
-    return lo;
+#pragma unroll
+        for (int o = 1; o < TP; o <<= 1) {
+            c += __shfl_xor_sync(0xffffffffu, c, o);
+            m += __shfl_xor_sync(0xffffffffu, m, o);
+        }
+        return pack(c, m);
+    };
+    const u64 base = shi;
+    const u64 at_mine = base + sums(mine, false);   // by every thread: its shuffles need whole warps
+    const uint32_t t = max(lo, row.max32(mine >= lo && ok(at_mine) ? mine : 0u));
+    slo = base + sums(t, false);
+    shi = base + sums(t, true);
+    return t;
 }
 
 template <int DT, int NT, int CL>
-__global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kernel(const SampleArgs a) {
     typedef Row<NT, CL> R;
     constexpr int ES = DT == FL_F32 ? 4 : 2, VEC = 16 / ES, J = kTok / VEC;
     __shared__ typename R::Shared shared;
@@ -204,41 +258,46 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
     const int r = blockIdx.x / CL;
     const char* l = static_cast<const char*>(a.logits) + (size_t)r * a.ld * ES;
     const int i0 = row.rank * a.seg, i1 = min(a.V, i0 + a.seg);   // this CTA's tokens
-    // token of (group j, element e) of this thread: its groups of VEC tokens
-    // begin on 16-byte boundaries, the first at or before token i0
-    const int first = i0 - (int)(((uintptr_t)l + (size_t)i0 * ES) % 16) / ES + (int)threadIdx.x * VEC;
-    auto token = [&](int j, int e) { return first + j * (NT * VEC) + e; };
+    // token of (group j, element e) of this thread: a warp's tokens are a
+    // contiguous piece, groups of VEC begin on 16-byte boundaries, the first
+    // of the CTA at or before token i0
+    const int first = i0 - (int)(((uintptr_t)l + (size_t)i0 * ES) % 16) / ES + row.warp * (32 * kTok) + row.lane * VEC;
+    auto token = [&](int j, int e) { return first + j * (32 * VEC) + e; };
 
-    uint32_t w[kTok];   // logits as sortable keys, then weights
-    uint32_t kmax = 0;
+    uint32_t w[kTok];   // logits, then weights
+    const int w0 = token(0, 0) - row.lane * VEC;   // this warp's tokens
+    if (w0 >= i0 && w0 + 32 * kTok <= i1) {
+        uint4 q[J];   // all loads in flight at once
 #pragma unroll
-    for (int j = 0; j < J; j++) {
-        const int t0 = token(j, 0);
-        if (t0 >= i0 && t0 + VEC <= i1) {
-            const uint4 q = *reinterpret_cast<const uint4*>(l + (size_t)t0 * ES);
-            const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+        for (int j = 0; j < J; j++) q[j] = *reinterpret_cast<const uint4*>(l + (size_t)token(j, 0) * ES);
+#pragma unroll
+        for (int j = 0; j < J; j++) {
+            const uint32_t qw[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                float x;
-                if constexpr (DT == FL_F32) x = __uint_as_float(qw[e]);
+                if constexpr (DT == FL_F32) w[j * VEC + e] = qw[e];
                 else if constexpr (DT == FL_F16) {
                     const __half2 h = *reinterpret_cast<const __half2*>(&qw[e >> 1]);
-                    x = (e & 1) ? __high2float(h) : __low2float(h);
-                } else x = __uint_as_float((e & 1) ? qw[e >> 1] & 0xffff0000u : qw[e >> 1] << 16);
-                w[j * VEC + e] = sortable(canon(x));
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const int t = t0 + e;
-                w[j * VEC + e] = sortable(t >= i0 && t < i1 ? logit<DT>(l, t) : -INFINITY);
+                    w[j * VEC + e] = __float_as_uint((e & 1) ? __high2float(h) : __low2float(h));
+                } else w[j * VEC + e] = (e & 1) ? qw[e >> 1] & 0xffff0000u : qw[e >> 1] << 16;
             }
         }
+    } else {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) kmax = max(kmax, w[j * VEC + e]);
+        for (int i = 0; i < kTok; i++) {
+            const int t = token(i / VEC, i % VEC);
+            w[i] = __float_as_uint(t >= i0 && t < i1 ? logit<DT>(l, t) : -INFINITY);
+        }
     }
-    kmax = row.max32(kmax);
-    const float mx = unsortable(kmax);
+    float mx = -INFINITY;   // NaN is never the larger
+#pragma unroll
+    for (int i = 0; i < kTok; i++) mx = fmaxf(mx, __uint_as_float(w[i]));
+    mx = unsortable(row.max32(sortable(mx)));
+    if (mx == INFINITY) {
+        mx = FLT_MAX;
+#pragma unroll
+        for (int i = 0; i < kTok; i++) w[i] = __float_as_uint(canon(__uint_as_float(w[i])));
+    }
     const float T = a.temperature ? a.temperature[r] : 1.0f;
     if (mx == -INFINITY || !(T > 0.0f)) {
         uint32_t best = 0;   // complement of the lowest index with the largest logit
@@ -246,7 +305,7 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int e = 0; e < VEC; e++)
-                if (w[j * VEC + e] == kmax && token(j, e) >= i0 && token(j, e) < i1)
+                if (__uint_as_float(w[j * VEC + e]) == mx && token(j, e) >= i0 && token(j, e) < i1)
                     best = max(best, ~(uint32_t)token(j, e));
         best = row.max32(best);
         if (row.rank == 0 && threadIdx.x == 0) a.tokens[r] = mx == -INFINITY ? -1 : (int)~best;
@@ -261,16 +320,16 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
         const float rt = __frcp_rn(T), low = -18.0f * T;
 #pragma unroll
         for (int i = 0; i < kTok; i++) {
-            const float x = __fsub_rn(unsortable(w[i]), mx);
-            const float q0 = __fmul_rn(x, rt);
-            const float q = __fmaf_rn(__fmaf_rn(-q0, T, x), rt, q0);
-            w[i] = x > low ? sample_weight(q) : 0u;
+            const float x = __fsub_rn(__uint_as_float(w[i]), mx);
+            const float xc = fmaxf(x, low);   // its weight is 0 too, and its quotient in range
+            const float q0 = __fmul_rn(xc, rt);
+            w[i] = sample_weight(__fmaf_rn(__fmaf_rn(-q0, T, xc), rt, q0)) + kTag;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kTok; i++) w[i] = sample_weight(__fdiv_rn(__fsub_rn(unsortable(w[i]), mx), T));
+        for (int i = 0; i < kTok; i++) w[i] = sample_weight(__fdiv_rn(__fsub_rn(__uint_as_float(w[i]), mx), T)) + kTag;
     }
-    const u64 all = row.sum(at_least(w, 1u));
+    const u64 all = at_least(row, w, 1u);
     u64 slo = all, shi = 0;
     uint32_t lo = 1u;          // kept: the weights >= lo
     u64 z = all & kMass;
@@ -285,8 +344,8 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
     const uint32_t kth = ties > room ? lo : 0u;   // the weight of which only some are kept
     const float tp = a.top_p ? a.top_p[r] : 1.0f;
     if (tp < 1.0f) {
-        const u128 need = (u128)max(1u, fixed24(tp)) * z;
-        auto ok = [&](u64 s) { return ((u128)(s & kMass) << 24) >= need; };
+        const u64 need = (u64)(((u128)max(1u, fixed24(tp)) * z + (kOne - 1u)) >> 24);
+        auto ok = [&](u64 s) { return (s & kMass) >= need; };
         // after top-k within the weights above the k-th, which are all kept, if they suffice
         if (ties == 0 || ok(shi)) {
             if (ties) slo = shi;
@@ -296,89 +355,60 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
     }
     if (a.min_p) lo = max(lo, fixed24(a.min_p[r]));
 
-    // The first token, in order, at which the running sum of f(i, token)
-    // exceeds target(total); to_all: the index goes to every thread.
-    auto locate = [&](auto f, auto target, bool to_all) __attribute__((always_inline)) -> uint32_t {
-        u64 own = 0;
+    // The first token, in order, at which the running sum of the values that
+    // f(sum, i, token, t) adds exceeds target(total); the values may carry the
+    // tag. to_all: the index goes to every thread.
+    auto locate = [&](uint32_t t, auto f, auto target, bool to_all) __attribute__((always_inline)) -> uint32_t {
+        uint32_t own = 0;
 #pragma unroll
         for (int j = 0; j < J; j++) {
-            uint32_t c = 0;
+            uint32_t g = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; e++) c += f(j * VEC + e, token(j, e));
-            const u64 s = warp_sum64(c);
-            if (row.lane == 0) shared.cell[j * R::NW + row.warp] = s;
-            own += c;
+            for (int e = 0; e < VEC; e++) f(g, j * VEC + e, token(j, e), t);
+            own += g & (kTag - 1u);
         }
-        // total, and the sum of the CTAs before this one
-        row.push(warp_sum64(own));
-        if (CL == 1) row.sync(); else { __syncthreads(); row.sync(); }
-        u64 tot = 0, before = 0;
+        const u64* s = row.share(warp_pack(0, own));
+        u64 tot = 0, c = 0, mine = 0;
 #pragma unroll
-        for (int i = 0; i < CL * R::NW; i += 32)
-            if (i + row.lane < CL * R::NW) {
-                const u64 s = shared.slot[row.phase][i + row.lane];
-                tot += s;
-                before += i + row.lane < row.rank * R::NW ? s : 0;
-            }
-        row.phase ^= 1;
-        tot = warp_sum64(tot);
-        before = warp_sum64(before);
+        for (int i = 0; i < R::NS; i++) {
+            tot += s[i];
+            c += i < row.me ? s[i] : 0;
+            mine = i == row.me ? s[i] : mine;
+        }
         const u64 tgt = target(tot);
-        // the cell: lane n takes the cells [n PC, (n + 1) PC)
-        constexpr int CELLS = J * R::NW, PC = (CELLS + 31) / 32;
-        u64 inc = 0;
-#pragma unroll
-        for (int i = 0; i < PC; i++) inc += row.lane * PC + i < CELLS ? shared.cell[row.lane * PC + i] : 0;
-        const u64 mine = inc;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-            if (row.lane >= o) inc += y;
-        }
-        u64 c = before + inc - mine;
-        int cell = -1;
-        for (int i = 0; i < PC; i++) {
-            const u64 s = row.lane * PC + i < CELLS ? shared.cell[row.lane * PC + i] : 0;
-            if (cell < 0) {
-                if (c <= tgt && tgt < c + s) cell = row.lane * PC + i;
-                else c += s;
-            }
-        }
-        const uint32_t who = __ballot_sync(0xffffffffu, cell >= 0);
         uint32_t res = 0;   // complement of the index
-        if (who) {
-            const int src = __ffs(who) - 1;
-            cell = __shfl_sync(0xffffffffu, cell, src);
-            c = __shfl_sync(0xffffffffu, c, src);
-            if (cell % R::NW == row.warp) {
-                uint32_t f4[VEC] = {}, sum = 0;
-                int t0 = 0;
+        again(t);
+        if (c <= tgt && tgt < c + mine) {   // this warp's piece: group by group
+            bool found = false;
 #pragma unroll
-                for (int j = 0; j < J; j++) {   // selects: an index of run time would move w to local memory
-                    const bool here = j == cell / R::NW;
-                    t0 = here ? token(j, 0) : t0;
+            for (int j = 0; j < J; j++) {
+                uint32_t v[VEC], g = 0;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        const uint32_t v = f(j * VEC + e, token(j, e));
-                        f4[e] = here ? v : f4[e];
+                for (int e = 0; e < VEC; e++) {
+                    v[e] = 0;
+                    f(v[e], j * VEC + e, token(j, e), t);
+                    v[e] &= kTag - 1u;
+                    g += v[e];
+                }
+                const u64 all_g = warp_pack(0, g);
+                if (!found && tgt < c + all_g) {
+                    found = true;
+                    u64 run = g;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const u64 y = __shfl_up_sync(0xffffffffu, run, o);
+                        if (row.lane >= o) run += y;
+                    }
+                    u64 b = c + run - g;
+                    if (b <= tgt && tgt < b + g) {
+#pragma unroll
+                        for (int e = 0; e < VEC; e++) {
+                            if (res == 0 && tgt < b + v[e]) res = ~(uint32_t)token(j, e);
+                            b += v[e];
+                        }
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < VEC; e++) sum += f4[e];
-                u64 run = sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 y = __shfl_up_sync(0xffffffffu, run, o);
-                    if (row.lane >= o) run += y;
-                }
-                u64 b = c + run - sum;
-                if (b <= tgt && tgt < b + sum) {
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        if (res == 0 && tgt < b + f4[e]) res = ~(uint32_t)(t0 + e);
-                        b += f4[e];
-                    }
-                }
+                c += all_g;
             }
         }
         if (to_all) return ~row.max32(res);
@@ -394,7 +424,7 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int e = 0; e < VEC; e++)
-                if (w[j * VEC + e] == kth) {
+                if (w[j * VEC + e] == kth + kTag) {
                     const uint32_t s = sortable(logit<DT>(l, token(j, e)));
                     top = max(top, s);
                     bot = max(bot, ~s);
@@ -402,13 +432,13 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
         top = row.max32(top);
         bot = ~row.max32(bot);
         auto key_count = [&](uint32_t t) {   // ties with a key of at least t
-            u64 c = 0;
+            uint32_t c = 0;
 #pragma unroll
             for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
-                    if (w[j * VEC + e] == kth) c += sortable(logit<DT>(l, token(j, e))) >= t;
-            return row.sum(c);
+                    if (w[j * VEC + e] == kth + kTag) c += sortable(logit<DT>(l, token(j, e))) >= t;
+            return row.sum(0, c);
         };
         // bot: the largest key with `room` ties at or above it
         uint32_t up = top + 1u;
@@ -418,19 +448,21 @@ __global__ void __launch_bounds__(NT) sample_rows_kernel(const SampleArgs a) {
             const u64 c = key_count(mid);
             if (c >= room) bot = mid; else { up = mid; above = c; }
         }
-        auto equal = [&](int i, int t) -> uint32_t { return w[i] == kth && sortable(logit<DT>(l, t)) == bot; };
-        const uint32_t last = locate(equal, [&](u64) { return room - above - 1; }, true);
+        auto equal = [&](uint32_t& sum, int i, int n, uint32_t t) {
+            if (w[i] == t) sum += sortable(logit<DT>(l, n)) == bot;
+        };
+        const uint32_t last = locate(kth + kTag, equal, [&](u64) { return room - above - 1; }, true);
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int e = 0; e < VEC; e++)
-                if (w[j * VEC + e] == kth) {
+                if (w[j * VEC + e] == kth + kTag) {
                     const uint32_t s = sortable(logit<DT>(l, token(j, e)));
-                    if (s < bot || (s == bot && (uint32_t)token(j, e) > last)) w[j * VEC + e] = 0u;
+                    if (s < bot || (s == bot && (uint32_t)token(j, e) > last)) w[j * VEC + e] = kTag;
                 }
     }
     const uint32_t U = min(fixed24(a.u[r]), kOne - 1u);
-    locate([&](int i, int) -> uint32_t { return w[i] >= lo ? w[i] : 0u; },
+    locate(lo + kTag, [&](uint32_t& sum, int i, int, uint32_t t) { add_if_ge(sum, w[i], t, row.one); },
            [&](u64 total) { return (u64)(((u128)U * total) >> 24); }, false);
 }
 
@@ -450,27 +482,33 @@ cudaError_t launch_sample(const SampleArgs& a, int rows, cudaStream_t s) {
 }
 
 // Tokens a CTA holds: its first group may begin up to 7 tokens early.
-constexpr int kSmall = 256, kLarge = 1024;
 constexpr int cta_tokens(int threads) { return threads * kTok - 8; }
-constexpr int kMaxVocab = 262000;   // eight CTAs
+constexpr int kMaxVocab = 262000;   // eight CTAs of 512 threads
+
+int sample_sms() {
+    static const int sms = [] {
+        int dev = 0, n = 0;
+        cudaGetDevice(&dev);
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        return n > 0 ? n : 148;
+    }();
+    return sms;
+}
 
 template <int DT>
 cudaError_t sample_dt(SampleArgs a, int rows, cudaStream_t s) {
-    const int V = a.V;
-    auto seg = [&](int cl) { return ((V + cl - 1) / cl + 7) / 8 * 8; };
-    int cl = 1;
-    if (V <= cta_tokens(kSmall)) {
-        a.seg = seg(1);
-        return launch_sample<DT, kSmall, 1>(a, rows, s);
-    }
-    while (seg(cl) > cta_tokens(kLarge)) cl *= 2;
-    a.seg = seg(cl);
-    switch (cl) {
-        case 1: return launch_sample<DT, kLarge, 1>(a, rows, s);
-        case 2: return launch_sample<DT, kLarge, 2>(a, rows, s);
-        case 4: return launch_sample<DT, kLarge, 4>(a, rows, s);
-        default: return launch_sample<DT, kLarge, 8>(a, rows, s);
-    }
+    // a cluster of cl CTAs of `threads` that covers a row
+    auto fits = [&](int threads, int cl) {
+        a.seg = ((a.V + cl - 1) / cl + 7) / 8 * 8;
+        return a.seg <= cta_tokens(threads);
+    };
+    if (fits(128, 1)) return launch_sample<DT, 128, 1>(a, rows, s);
+    // few rows: more SMs a row
+    if (rows * 4 <= sample_sms() * SAMPLE_FEW && fits(128, 4)) return launch_sample<DT, 128, 4>(a, rows, s);
+    if (fits(512, 1)) return launch_sample<DT, 512, 1>(a, rows, s);
+    if (fits(256, 8)) return launch_sample<DT, 256, 8>(a, rows, s);
+    if (fits(512, 8)) return launch_sample<DT, 512, 8>(a, rows, s);
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace
