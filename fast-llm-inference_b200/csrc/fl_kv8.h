@@ -36,28 +36,21 @@ __host__ __device__ __forceinline__ int kv8_v_off(int pos, int d) {
     return (d >> 5) * 512 + ((d & 31) >> 2) * 64 + (pos >> 2) * 16 + (d & 3) * 4 + (pos & 3);
 }
 
-// One work item of the attention: a tile of packed query rows of a sequence
-// (packed row p: token p / group, query head kv_head * group + p % group)
-// over a range of its pages.
-struct Kv8Item {
-    int seq, tile, page0, pages;
-    int split, splits;   // this range among the tile's; 1 = the whole context
-    int part;            // first partial slot of the tile (splits > 1)
-    int pad;
-};
-
 // Counts and constants that a plan leaves on the device.
 struct Kv8Meta {
-    int seqs, rows, units, gblocks, items, pad[3];
+    int seqs, rows, units, gblocks;
+    int refused;             // the plan changed nothing
+    int max_pages;           // of a sequence with new rows
+    long long tiles, work;   // row tiles of the attention, (row tile, page) pairs, per kv head
 };
 
 // Device arrays of a plan (all owned by the handle).
 struct Kv8Tables {
     int *block_table, *held, *free_pages, *n_free, *row_start, *kv_start, *slot, *pos, *row_seq, *status;
     int *ctx;          // [max_seqs] cached positions of the planned sequences
-    int *take_start, *rel_start, *unit_start, *gblk_start, *item_start, *part_start;  // [max_seqs + 1]
+    int *take_start, *rel_start, *unit_start, *gblk_start;  // [max_seqs + 1]
+    long long *tile_start, *work_start;   // [max_seqs + 1] row tiles, (row tile, page) pairs before each
     int *unit_row;     // [max_rows] first row of every (sequence, 16-position block) touched
-    Kv8Item* items;
     Kv8Meta* meta;
 };
 
@@ -68,16 +61,16 @@ struct fl_kv8 {
     int device = 0, sms = 148;
     int max_pages = 0;          // pages per sequence
     int group = 1, tile_rows = 16;
-    int items_cap = 0, parts_cap = 0, target = 0;
+    int parts = 0;              // CTAs of an attention launch
     int max_new = 0;            // bound of the last plan
     int nseq = 0;
     std::vector<void*> bufs;
     std::vector<uint8_t*> k, v;       // [layers] codes
     std::vector<float*> ks, vs;       // [layers] scales
     fl::Kv8Tables t = {};
-    float* part = nullptr;      // [parts][kv_heads][tile_rows][head_dim] partial outputs
-    float2* part_ml = nullptr;  // [parts][kv_heads][tile_rows] (maximum, sum)
-    int* part_cnt = nullptr;    // [parts][kv_heads] arrivals, zero between launches
+    float* part = nullptr;      // [2 parts][tile_rows][head_dim] partial outputs
+    float2* part_ml = nullptr;  // [2 parts][tile_rows] (maximum, sum)
+    int* part_cnt = nullptr;    // [parts] arrivals, zero between launches
 };
 
 namespace fl {

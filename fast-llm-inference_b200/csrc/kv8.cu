@@ -28,7 +28,7 @@ struct PlanArgs {
     const int *ctx, *nw;
     Kv8Tables t;
     int nseq, max_new, max_pages, max_rows;
-    int group, tile_rows, kv_heads, target;
+    int group, tile_rows;
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -56,6 +56,37 @@ __device__ int block_scan(int v, int* red, int* total) {
     *total = __shfl_sync(0xffffffffu, w, 31);
     const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
     return (warp ? before : 0) + inc - v;
+}
+
+// The same of 64-bit numbers.
+__device__ long long block_scan64(long long v, long long* red, long long* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();
+    if (lane == 31) red[warp] = inc;
+    __syncthreads();
+    long long w = red[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+    }
+    *total = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    return (warp ? before : 0) + inc - v;
+}
+
+__device__ int block_max(int v, int* red) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, red[threadIdx.x & 31]);
 }
 
 __device__ long long block_sum64(long long v, long long* red) {
@@ -134,11 +165,11 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
         if (threadIdx.x == 0) *t.status = st;
         if (st != 0) {
             for (int b = threadIdx.x; b <= a.nseq; b += kPT) t.row_start[b] = t.kv_start[b] = 0;
-            if (threadIdx.x == 0) *t.meta = Kv8Meta{a.nseq, 0, 0, 0, 0, {1, 0, 0}};
+            if (threadIdx.x == 0) *t.meta = Kv8Meta{a.nseq, 0, 0, 0, 1, 0, 0, 0};
         } else {
             // sums of this thread's sequences, then the prefixes
             int v[6] = {};
-            long long w = 0;   // (row tile, page) pairs: the attention's work
+            long long w = 0, nt = 0;   // (row tile, page) pairs, row tiles: the attention's work
             for (int b = b0; b < b1; b++) {
                 const SeqPlan s = seq_plan(a, b);
                 const int n = s.n ? s.ctx + s.n : 0;
@@ -148,26 +179,22 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
                 v[3] += s.need - s.keep;
                 v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
                 v[5] += (n + kKv8Block - 1) / kKv8Block;
-                w += (long long)((s.n * a.group + a.tile_rows - 1) / a.tile_rows) * ((n + kPageSize - 1) / kPageSize);
+                const int tl = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
+                nt += tl;
+                w += (long long)tl * ((n + kPageSize - 1) / kPageSize);
             }
             int tot[6];
 #pragma unroll
             for (int i = 0; i < 6; i++) v[i] = block_scan(v[i], red, &tot[i]);
-            w = block_sum64(w, red64);
-            // pages per item: as few as make about `target` items over all heads
-            const long long want = max(1, a.target / a.kv_heads);
-            const int per = (int)max(1ll, (w + want - 1) / want);
-            int ni = 0, np = 0, toti, totp;
+            long long totw, tott;
+            w = block_scan64(w, red64, &totw);
+            nt = block_scan64(nt, red64, &tott);
+            int mp = 0;
             for (int b = b0; b < b1; b++) {
                 const SeqPlan s = seq_plan(a, b);
-                if (!s.n) continue;
-                const int tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
-                const int pages = (s.ctx + s.n + kPageSize - 1) / kPageSize, sp = (pages + per - 1) / per;
-                ni += tiles * sp;
-                np += sp > 1 ? tiles * sp : 0;
+                mp = max(mp, s.n ? (s.ctx + s.n + kPageSize - 1) / kPageSize : 0);
             }
-            ni = block_scan(ni, red, &toti);
-            np = block_scan(np, red, &totp);
+            mp = block_max(mp, red);
             for (int b = b0; b < b1; b++) {
                 const SeqPlan s = seq_plan(a, b);
                 const int n = s.n ? s.ctx + s.n : 0;
@@ -178,20 +205,17 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
                 t.take_start[b] = v[3];
                 t.unit_start[b] = v[4];
                 t.gblk_start[b] = v[5];
-                t.item_start[b] = ni;
-                t.part_start[b] = np;
+                t.tile_start[b] = nt;
+                t.work_start[b] = w;
                 v[0] += s.n;
                 v[1] += n;
                 v[2] += s.rel;
                 v[3] += s.need - s.keep;
                 v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
                 v[5] += (n + kKv8Block - 1) / kKv8Block;
-                if (s.n) {
-                    const int tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
-                    const int pages = (n + kPageSize - 1) / kPageSize, sp = (pages + per - 1) / per;
-                    ni += tiles * sp;
-                    np += sp > 1 ? tiles * sp : 0;
-                }
+                const int tl = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
+                nt += tl;
+                w += (long long)tl * ((n + kPageSize - 1) / kPageSize);
             }
             if (threadIdx.x == 0) {
                 t.row_start[a.nseq] = tot[0];
@@ -200,15 +224,14 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
                 t.take_start[a.nseq] = tot[3];
                 t.unit_start[a.nseq] = tot[4];
                 t.gblk_start[a.nseq] = tot[5];
-                t.item_start[a.nseq] = toti;
-                t.part_start[a.nseq] = totp;
-                *t.meta = Kv8Meta{a.nseq, tot[0], tot[4], tot[5], toti, {0, per, 0}};
+                t.tile_start[a.nseq] = tott;
+                t.work_start[a.nseq] = totw;
+                *t.meta = Kv8Meta{a.nseq, tot[0], tot[4], tot[5], 0, mp, tott, totw};
             }
         }
     }
     cluster_sync();
-    if (__ldcg(&t.meta->pad[0])) return;   // refused: nothing changes (every CTA alike)
-    const int per = __ldcg(&t.meta->pad[1]);
+    if (__ldcg(&t.meta->refused)) return;   // nothing changes (every CTA alike)
     const int nfree = __ldcg(t.n_free), top = nfree + __ldcg(t.rel_start + a.nseq);
     const int lane = threadIdx.x & 31;
     const int wid = (int)rank * (kPT / 32) + (threadIdx.x >> 5), nw = (int)nrank * (kPT / 32);
@@ -234,16 +257,6 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
         const int units = (n - 1) / kKv8Block - s.ctx / kKv8Block + 1;
         for (int u = lane; u < units; u += 32)
             t.unit_row[u0 + u] = r0 + (u ? u * kKv8Block - s.ctx % kKv8Block : 0);
-        const int tiles = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
-        const int pages = (n + kPageSize - 1) / kPageSize, sp = (pages + per - 1) / per;
-        const int i0 = __ldcg(t.item_start + b), p0 = __ldcg(t.part_start + b);
-        for (int i = lane; i < tiles * sp; i += 32) {
-            const int tile = i / sp, k = i - tile * sp;
-            // even shares: the first pages % sp ranges are one page longer
-            const int base = pages / sp, rem = pages - base * sp;
-            t.items[i0 + i] = Kv8Item{b, tile, k * base + min(k, rem), base + (k < rem ? 1 : 0),
-                                      k, sp, sp > 1 ? p0 + tile * sp : 0, 0};
-        }
     }
     cluster_sync();
     if (rank == 0 && threadIdx.x == 0) *t.n_free = top - __ldcg(t.take_start + a.nseq);
@@ -534,7 +547,7 @@ int create(fl_kv8* h) {
     h->group = c.heads / c.kv_heads;
     h->tile_rows = c.dtype == FL_F32 ? 8 : 16;
     cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device);
-    h->target = h->sms * kv8_attention_occupancy(c.head_dim, c.type, c.dtype);
+    h->parts = h->sms * kv8_attention_occupancy(c.head_dim, c.type, c.dtype);
     const size_t S = c.max_seqs, R = c.max_rows, kvb = (size_t)c.pages * c.kv_heads * kPageSize * c.head_dim;
     h->k.resize(c.layers);
     h->v.resize(c.layers);
@@ -556,22 +569,15 @@ int create(fl_kv8* h) {
     FL_CHECK(alloc(h, &t.pos, R, true));
     FL_CHECK(alloc(h, &t.row_seq, R, true));
     FL_CHECK(alloc(h, &t.unit_row, R, true));
-    for (int** p : {&t.row_start, &t.kv_start, &t.take_start, &t.rel_start, &t.unit_start, &t.gblk_start, &t.item_start,
-                    &t.part_start, &t.ctx})
+    for (int** p : {&t.row_start, &t.kv_start, &t.take_start, &t.rel_start, &t.unit_start, &t.gblk_start, &t.ctx})
         FL_CHECK(alloc(h, p, S + 1, true));
-    // a plan makes at most target / kv_heads items beyond one a tile, and
-    // splits only tiles of more pages than an item takes: at most twice that
-    // many partial results
-    const size_t want = std::max(1, h->target / c.kv_heads);
-    const size_t tiles = (R * h->group + h->tile_rows - 1) / h->tile_rows + S;
-    h->items_cap = (int)(tiles + want);
-    h->parts_cap = (int)(2 * want);
-    FL_CHECK(alloc(h, &t.items, h->items_cap, false));
+    FL_CHECK(alloc(h, &t.tile_start, S + 1, true));
+    FL_CHECK(alloc(h, &t.work_start, S + 1, true));
     FL_CHECK(alloc(h, &t.meta, 1, true));
-    const size_t np = (size_t)h->parts_cap * c.kv_heads;
-    FL_CHECK(alloc(h, &h->part, np * h->tile_rows * c.head_dim, false));
-    FL_CHECK(alloc(h, &h->part_ml, np * h->tile_rows, false));
-    FL_CHECK(alloc(h, &h->part_cnt, np, true));
+    // a part begins inside a tile at most, and ends inside one
+    FL_CHECK(alloc(h, &h->part, (size_t)2 * h->parts * h->tile_rows * c.head_dim, false));
+    FL_CHECK(alloc(h, &h->part_ml, (size_t)2 * h->parts * h->tile_rows, false));
+    FL_CHECK(alloc(h, &h->part_cnt, h->parts, true));
     kv8_reset_kernel<<<64, 256>>>(t, c.pages, c.max_seqs);
     FL_CHECK_CUDA(cudaGetLastError());
     FL_CHECK_CUDA(cudaDeviceSynchronize());
@@ -673,8 +679,6 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     a.max_rows = h->c.max_rows;
     a.group = h->group;
     a.tile_rows = h->tile_rows;
-    a.kv_heads = h->c.kv_heads;
-    a.target = h->target;
     // one CTA while its threads hold the rows; eight (a portable cluster) beyond
     const long long rows = std::min<long long>((long long)nseq * a.max_new, h->c.max_rows);
     cudaLaunchConfig_t cfg = {};
@@ -787,6 +791,6 @@ FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, in
     p.part = h->part;
     p.part_ml = h->part_ml;
     p.part_cnt = h->part_cnt;
-    FL_CHECK_CUDA(launch_kv8_attention(p, h->target, s));
+    FL_CHECK_CUDA(launch_kv8_attention(p, h->parts, s));
     return FL_OK;
 }

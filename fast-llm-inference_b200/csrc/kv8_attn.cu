@@ -18,6 +18,8 @@
 // probabilities of f32 rows are split the same way.
 #include <math.h>
 
+#include <algorithm>
+
 #include "fl_common.cuh"
 #include "fl_kv8.h"
 #include "fl_kv8_types.cuh"
@@ -27,6 +29,8 @@ namespace fl {
 namespace {
 
 constexpr int kAW = 4;   // warps per CTA: one per 16-position block of a page
+constexpr int kStages = 4;   // blocks in flight or in use per warp
+constexpr float kTileCost = 3.0f, kJoinCost = 20.0f;   // in pages, see the kernel
 constexpr float kShift = 7.0f;   // probabilities enter as 2^7 p: 2^-21 of the largest is a normal half
 constexpr float kSlack = 8.0f;   // the reference follows the maximum once it lags by 2^8
 
@@ -59,6 +63,23 @@ __device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t& lo, uint32
     }
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 lds8(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+
 // 8 values at dimensions d .. d + 7 of a query row.
 template <int DT>
 __device__ __forceinline__ void load8(const void* q, size_t i, int vec, float (&f)[8]) {
@@ -72,6 +93,76 @@ __device__ __forceinline__ void load8(const void* q, size_t i, int vec, float (&
     }
 }
 
+// A range of a tile's pages.
+struct Kv8Item {
+    int seq, head, ctx, row0, nb;
+    int tile, page0, pages;   // no pages: none is left
+    int split, splits;        // this range among the tile's
+    int part;                 // the part that holds the tile's first page
+    long long next;           // where the CTA goes on
+};
+
+// The sequence whose work x falls into: start[b] <= x < start[b + 1]. A warp
+// narrows the range 32-fold a step.
+__device__ __forceinline__ int find_work(const long long* start, int nseq, long long x, int lane) {
+    int lo = 0, n = nseq;   // start[lo] <= x < start[lo + n]
+    while (n > 1) {
+        const int step = (n + 31) / 32;
+        const int at = lo + lane * step;
+        const bool below = lane * step < n && start[at] <= x;
+        const int k = 31 - __clz((int)__ballot_sync(0xffffffffu, below));
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return lo;
+}
+
+// The work of a CTA, item by item (x: where it stands, -1 at first); by a warp.
+// Two ways to share it. Whole tiles, CTA by CTA; or the (kv head, row tile,
+// page) triples, in that order, cut into equal parts, one a CTA, which end
+// together whatever the lengths are, while a tile that several parts share is
+// joined by the last of them to arrive. What each takes is estimated in pages:
+// kTileCost a tile, kJoinCost for the joins. At 64 x 32 tiles of 21 pages whole
+// tiles took 106 us and parts 120; at 24 x 10 tiles of 5 to 500, 290 and 168.
+__device__ __forceinline__ void next_item(const Kv8AttnParams& p, long long x, int lane, Kv8Item& out) {
+    const Kv8Meta& mt = *p.t.meta;
+    const long long tiles = mt.tiles, work = mt.work, G = gridDim.x;
+    const float mean = (float)work / (float)max(1ll, tiles), per_cta = (float)(tiles * p.kv_heads) / (float)G;
+    const bool whole = ceilf(per_cta) * (mean + kTileCost) + ((float)mt.max_pages - mean) <=
+                       per_cta * mean + (per_cta + 1.0f) * kTileCost + kJoinCost;
+    const long long total = (whole ? tiles : work) * p.kv_heads;
+    const long long size = whole ? 1 : (total + G - 1) / G;
+    if (x < 0) x = (long long)blockIdx.x * size;
+    Kv8Item it = {};
+    if (x < (whole ? total : min(total, (blockIdx.x + 1ll) * size))) {
+        it.head = (int)(x / (whole ? tiles : work));
+        const long long in_head = x - it.head * (whole ? tiles : work);
+        const long long* start = whole ? p.t.tile_start : p.t.work_start;
+        it.seq = find_work(start, mt.seqs, in_head, lane);
+        const long long in_seq = in_head - start[it.seq];
+        it.ctx = p.t.ctx[it.seq];
+        it.row0 = p.t.row_start[it.seq];
+        it.nb = p.t.row_start[it.seq + 1] - it.row0;
+        it.pages = (it.ctx + it.nb + kPageSize - 1) / kPageSize;
+        it.splits = 1;
+        if (whole) {
+            it.tile = (int)in_seq;
+            it.next = x + G;
+        } else {
+            const int tile_pages = it.pages;
+            it.tile = (int)(in_seq / tile_pages);
+            it.page0 = (int)(in_seq - (long long)it.tile * tile_pages);
+            it.pages = (int)min((long long)(tile_pages - it.page0), (blockIdx.x + 1ll) * size - x);
+            const long long tile_x = x - it.page0;   // the tile's first triple
+            it.part = (int)(tile_x / size);
+            it.splits = (int)((tile_x + tile_pages - 1) / size) - it.part + 1;
+            it.split = (int)blockIdx.x - it.part;
+            it.next = x + it.pages;
+        }
+    }
+    if (lane == 0) out = it;
+}
+
 // Shift of a row with largest magnitude a: a 2^sh in [2^14, 2^15); 0 for a
 // zero row and for one that is not finite (its results are NaN).
 __device__ __forceinline__ float row_shift(float a) {
@@ -81,22 +172,26 @@ __device__ __forceinline__ float row_shift(float a) {
 }
 
 template <int HD, int DT, bool E4M3>
-__global__ void __launch_bounds__(kAW * 32) kv8_attention_kernel(const Kv8AttnParams p, const int vec) {
+__global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8AttnParams p, const int vec) {
     constexpr bool F32 = DT == FL_F32;
     constexpr int TR = F32 ? 8 : 16;   // query rows per tile
     constexpr int NC = HD / 32;
     constexpr int RR = F32 ? 1 : 2;    // rows of a thread
-    __shared__ float o_s[kAW][TR][HD];
+    constexpr int kStage = 2 * NC * 512 + 16;   // bytes: K, V, the two scales
+    extern __shared__ __align__(128) uint8_t smem[];   // rings of the warps, then their results
+    float(*o_s)[TR][HD] = reinterpret_cast<float(*)[TR][HD]>(smem);
     __shared__ float m_s[kAW][TR], l_s[kAW][TR];
     __shared__ int last_s;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * kStage);
     const int g = lane >> 2, t4 = lane & 3;
-    const long long work = (long long)p.t.meta->items * p.kv_heads;
-    for (long long w = blockIdx.x; w < work; w += gridDim.x) {
-        const Kv8Item it = p.t.items[w / p.kv_heads];
-        const int h = (int)(w % p.kv_heads);
-        const int ctx = p.t.ctx[it.seq], row0 = p.t.row_start[it.seq];
-        const int nb = p.t.row_start[it.seq + 1] - row0;
+    __shared__ Kv8Item it;   // re-read where it is used: registers go to the tile
+    for (long long x = -1;;) {
+        if (warp == 0) next_item(p, x, lane, it);
+        __syncthreads();
+        if (it.pages == 0) break;
+        x = it.next;
+        const int h = it.head, ctx = it.ctx, row0 = it.row0, nb = it.nb;
         const int np = min(TR, nb * p.group - it.tile * TR);       // packed rows of the tile
         const int tok_last = (it.tile * TR + np - 1) / p.group;
         const int kend = p.mask ? ctx + nb : ctx + tok_last + 1;   // positions any row may see
@@ -163,18 +258,44 @@ __global__ void __launch_bounds__(kAW * 32) kv8_attention_kernel(const Kv8AttnPa
 #pragma unroll
                 for (int i = 0; i < 4; i++) o[c][j][i] = 0.0f;
 
+        // this warp's blocks: one a page, up to the last visible position. They
+        // pass through a ring in shared memory; every lane copies the very 16
+        // bytes that it will read, so a warp waits for its own copies alone
         const int* bt = p.t.block_table + (size_t)it.seq * p.max_pages + it.page0;
-        for (int i = 0; i < it.pages; i++) {
+        const int nblk = min(it.pages, (kend - it.page0 * kPageSize - warp * kKv8Block + kPageSize - 1) / kPageSize);
+        int pages = lane < nblk ? bt[lane] : 0;   // of 32 blocks at a time, one a lane
+        auto fetch = [&](int i) {
+            if (i < nblk) {
+                if (i && (i & 31) == 0) pages = i + lane < nblk ? bt[i + lane] : 0;
+                const size_t ph = (size_t)__shfl_sync(0xffffffffu, pages, i & 31) * p.kv_heads + h;
+                const size_t off = ph * (kPageSize * HD) + warp * (kKv8Block * HD) + lane * 16;
+                const uint32_t d = ring + (i % kStages) * kStage + lane * 16;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    cp_async16(d + c * 512, p.k + off + c * 512);
+                    cp_async16(d + (NC + c) * 512, p.v + off + c * 512);
+                }
+                if (lane < 2) cp_async4(ring + (i % kStages) * kStage + 2 * NC * 512 + lane * 4,
+                                        (lane ? p.vs : p.ks) + ph * kKv8Sub + warp);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; i++) fetch(i);
+        for (int i = 0; i < nblk; i++) {
             const int pos0 = (it.page0 + i) * kPageSize + warp * kKv8Block;
-            if (pos0 >= kend) break;
-            const size_t ph = (size_t)bt[i] * p.kv_heads + h;
-            const size_t off = ph * (kPageSize * HD) + warp * (kKv8Block * HD) + lane * 16;
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncwarp();   // the scales come from lanes 0 and 1; slot i - 1 has been read
+            const uint32_t st = ring + (i % kStages) * kStage;
             uint4 kq[NC], vq[NC];
 #pragma unroll
-            for (int c = 0; c < NC; c++) kq[c] = ld_stream16(p.k + off + c * 512);
-#pragma unroll
-            for (int c = 0; c < NC; c++) vq[c] = ld_stream16(p.v + off + c * 512);
-            const float ks = p.ks[ph * kKv8Sub + warp], vs = p.vs[ph * kKv8Sub + warp];
+            for (int c = 0; c < NC; c++) {
+                kq[c] = lds16(st + c * 512 + lane * 16);
+                vq[c] = lds16(st + (NC + c) * 512 + lane * 16);
+            }
+            const float2 sc = lds8(st + 2 * NC * 512);
+            const float ks = sc.x, vs = sc.y;
+            fetch(i + kStages - 1);
             // positions behind the sequence may hold anything: an E4M3 byte there may be a NaN
             if (E4M3 && pos0 + kKv8Block > ctx + nb) {
                 const int lim = ctx + nb - pos0 - 4 * t4;   // of this lane's four V positions
@@ -285,6 +406,7 @@ __global__ void __launch_bounds__(kAW * 32) kv8_attention_kernel(const Kv8AttnPa
             }
         }
         // this warp's result: reference, sum, normalised output
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < RR; r++) {
@@ -309,7 +431,8 @@ __global__ void __launch_bounds__(kAW * 32) kv8_attention_kernel(const Kv8AttnPa
         }
         __syncthreads();
         // joined over the warps: the weights are l 2^(m - M)
-        const size_t slot = (size_t)(it.part + it.split) * p.kv_heads + h;
+        // slots of a part: its first range, of a tile begun before it, and its last
+        const size_t slot = 2 * (size_t)blockIdx.x + (it.split == 0);
         for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kAW * 32) {
             const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
             float M = -INFINITY;
@@ -338,22 +461,21 @@ __global__ void __launch_bounds__(kAW * 32) kv8_attention_kernel(const Kv8AttnPa
         }
         if (it.splits > 1) {
             // the last range to arrive joins the tile's ranges, in their order
-            int* cnt = p.part_cnt + (size_t)it.part * p.kv_heads + h;
+            int* cnt = p.part_cnt + it.part;
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) last_s = atomicAdd(cnt, 1) == it.splits - 1;
             __syncthreads();
             if (last_s) {
                 __threadfence();
-                const size_t s0 = (size_t)it.part * p.kv_heads + h;
                 for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kAW * 32) {
                     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
                     float M = -INFINITY;
                     for (int k = 0; k < it.splits; k++)
-                        M = fmaxf(M, __ldcg(&p.part_ml[(s0 + (size_t)k * p.kv_heads) * TR + r]).x);
+                        M = fmaxf(M, __ldcg(&p.part_ml[(2 * (size_t)(it.part + k) + (k == 0)) * TR + r]).x);
                     float L = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
                     for (int k = 0; k < it.splits; k++) {
-                        const size_t sk = (s0 + (size_t)k * p.kv_heads) * TR + r;
+                        const size_t sk = (2 * (size_t)(it.part + k) + (k == 0)) * TR + r;
                         const float2 ml = __ldcg(&p.part_ml[sk]);
                         if (ml.y == 0.0f) continue;
                         const float wk = ml.y * exp2f(ml.x - M);
@@ -398,10 +520,19 @@ cudaError_t with_kernel(int hd, int type, int dtype, F f) {
 
 }  // namespace
 
+// Dynamic shared memory: the rings, later the warps' results.
+int attention_smem(int hd, int dtype) {
+    const int ring = kAW * kStages * (2 * (hd / 32) * 512 + 16);
+    return std::max(ring, kAW * (dtype == FL_F32 ? 8 : 16) * hd * 4);
+}
+
 int kv8_attention_occupancy(int head_dim, int type, int dtype) {
     int n = 0;
+    const int smem = attention_smem(head_dim, dtype);
     with_kernel(head_dim, type, dtype, [&](auto* k) {
-        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kAW * 32, 0);
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kAW * 32, smem);
+        return e;
     });
     return n > 0 ? n : 1;
 }
@@ -411,7 +542,7 @@ cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int ctas, cudaStream_t 
     const int vec = ((uintptr_t)p.q & 15) == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldq * es % 16 == 0 &&
                     p.ldo * es % 16 == 0;
     return with_kernel(p.head_dim, p.type, p.dtype, [&](auto* k) {
-        k<<<ctas, kAW * 32, 0, s>>>(p, vec);
+        k<<<ctas, kAW * 32, attention_smem(p.head_dim, p.dtype), s>>>(p, vec);
         return cudaGetLastError();
     });
 }
