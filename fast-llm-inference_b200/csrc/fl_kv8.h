@@ -15,6 +15,7 @@ namespace fl {
 
 constexpr int kKv8Block = FL_KV8_BLOCK;           // positions per scale
 constexpr int kKv8Sub = kPageSize / kKv8Block;    // scales per page and head
+constexpr int kKv8Long = 128;                     // packed query rows of a tile of the prefill kernel
 
 // Codes of one (page, kv head) are kPageSize * head_dim bytes: per block of
 // 16 positions, per chunk of 32 dimensions, 512 bytes in the order in which a
@@ -40,8 +41,13 @@ __host__ __device__ __forceinline__ int kv8_v_off(int pos, int d) {
 struct Kv8Meta {
     int seqs, rows, units, gblocks;
     int refused;             // the plan changed nothing
-    int max_pages;           // of a sequence with new rows
-    long long tiles, work;   // row tiles of the attention, (row tile, page) pairs, per kv head
+    int pad;
+    // the attention's two lists, of sequences with few and with many packed
+    // query rows (new rows x group): per kv head
+    struct List {
+        long long tiles, work;   // row tiles, (row tile, page) pairs
+        long long max_pages;     // of one of its sequences
+    } list[2];
 };
 
 // Device arrays of a plan (all owned by the handle).
@@ -49,7 +55,7 @@ struct Kv8Tables {
     int *block_table, *held, *free_pages, *n_free, *row_start, *kv_start, *slot, *pos, *row_seq, *status;
     int *ctx;          // [max_seqs] cached positions of the planned sequences
     int *take_start, *rel_start, *unit_start, *gblk_start;  // [max_seqs + 1]
-    long long *tile_start, *work_start;   // [max_seqs + 1] row tiles, (row tile, page) pairs before each
+    long long *tile_start[2], *work_start[2];   // [max_seqs + 1] of each list: tiles and pairs before a sequence
     int *unit_row;     // [max_rows] first row of every (sequence, 16-position block) touched
     Kv8Meta* meta;
 };
@@ -61,16 +67,16 @@ struct fl_kv8 {
     int device = 0, sms = 148;
     int max_pages = 0;          // pages per sequence
     int group = 1, tile_rows = 16;
-    int parts = 0;              // CTAs of an attention launch
+    int parts[2] = {};          // CTAs of an attention launch, of either list's kernel
     int max_new = 0;            // bound of the last plan
     int nseq = 0;
     std::vector<void*> bufs;
     std::vector<uint8_t*> k, v;       // [layers] codes
     std::vector<float*> ks, vs;       // [layers] scales
     fl::Kv8Tables t = {};
-    float* part = nullptr;      // [2 parts][tile_rows][head_dim] partial outputs
-    float2* part_ml = nullptr;  // [2 parts][tile_rows] (maximum, sum)
-    int* part_cnt = nullptr;    // [parts] arrivals, zero between launches
+    float* part[2] = {};        // [2 parts][rows of a tile][head_dim] partial outputs
+    float2* part_ml[2] = {};    // [2 parts][rows of a tile] (maximum, sum)
+    int* part_cnt[2] = {};      // [parts] arrivals, zero between launches
 };
 
 namespace fl {
@@ -87,12 +93,20 @@ struct Kv8AttnParams {
     float scale;         // of the scores, times log2(e)
     const uint8_t* mask; // [rows][ldm] or null: causal
     int ldm;
+};
+// One list's tiles and the workspace of its kernel.
+struct Kv8Tiles {
+    int list;
+    const long long *tile_start, *work_start;
     float* part;
     float2* part_ml;
     int* part_cnt;
 };
-cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int ctas, cudaStream_t s);
+cudaError_t launch_kv8_attention(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s);
+cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s);
 // CTAs of the attention kernel that one SM holds (for the plan's split).
 int kv8_attention_occupancy(int head_dim, int type, int dtype);
+int kv8_prefill_occupancy(int head_dim, int type, int dtype);
+int take_kv8_error();   // returns and clears the prefill kernel's error word
 
 }  // namespace fl

@@ -24,11 +24,18 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int kPT = 1024;
 
+// Packed query rows of a sequence (new rows x heads per kv head) from which the
+// prefill kernel takes it.
+#ifndef FL_KV8_LONG_MIN
+#define FL_KV8_LONG_MIN 40
+#endif
+constexpr int kLongMin = FL_KV8_LONG_MIN;
+
 struct PlanArgs {
     const int *ctx, *nw;
     Kv8Tables t;
     int nseq, max_new, max_pages, max_rows;
-    int group, tile_rows;
+    int group, tile_rows, long_min;   // packed rows from which a sequence is on the second list
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -165,11 +172,12 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
         if (threadIdx.x == 0) *t.status = st;
         if (st != 0) {
             for (int b = threadIdx.x; b <= a.nseq; b += kPT) t.row_start[b] = t.kv_start[b] = 0;
-            if (threadIdx.x == 0) *t.meta = Kv8Meta{a.nseq, 0, 0, 0, 1, 0, 0, 0};
+            if (threadIdx.x == 0) *t.meta = Kv8Meta{a.nseq, 0, 0, 0, 1, 0, {}};
         } else {
             // sums of this thread's sequences, then the prefixes
             int v[6] = {};
-            long long w = 0, nt = 0;   // (row tile, page) pairs, row tiles: the attention's work
+            long long w[2] = {}, nt[2] = {};   // the attention's lists
+            int mp[2] = {};
             for (int b = b0; b < b1; b++) {
                 const SeqPlan s = seq_plan(a, b);
                 const int n = s.n ? s.ctx + s.n : 0;
@@ -179,22 +187,22 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
                 v[3] += s.need - s.keep;
                 v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
                 v[5] += (n + kKv8Block - 1) / kKv8Block;
-                const int tl = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
-                nt += tl;
-                w += (long long)tl * ((n + kPageSize - 1) / kPageSize);
+                const int li = s.n * a.group >= a.long_min, tr = li ? kKv8Long : a.tile_rows;
+                const int tl = (s.n * a.group + tr - 1) / tr, pages = (n + kPageSize - 1) / kPageSize;
+                nt[li] += tl;
+                w[li] += (long long)tl * pages;
+                mp[li] = max(mp[li], pages);
             }
             int tot[6];
 #pragma unroll
             for (int i = 0; i < 6; i++) v[i] = block_scan(v[i], red, &tot[i]);
-            long long totw, tott;
-            w = block_scan64(w, red64, &totw);
-            nt = block_scan64(nt, red64, &tott);
-            int mp = 0;
-            for (int b = b0; b < b1; b++) {
-                const SeqPlan s = seq_plan(a, b);
-                mp = max(mp, s.n ? (s.ctx + s.n + kPageSize - 1) / kPageSize : 0);
+            long long totw[2], tott[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                w[i] = block_scan64(w[i], red64, &totw[i]);
+                nt[i] = block_scan64(nt[i], red64, &tott[i]);
+                mp[i] = block_max(mp[i], red);
             }
-            mp = block_max(mp, red);
             for (int b = b0; b < b1; b++) {
                 const SeqPlan s = seq_plan(a, b);
                 const int n = s.n ? s.ctx + s.n : 0;
@@ -205,17 +213,21 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
                 t.take_start[b] = v[3];
                 t.unit_start[b] = v[4];
                 t.gblk_start[b] = v[5];
-                t.tile_start[b] = nt;
-                t.work_start[b] = w;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    t.tile_start[i][b] = nt[i];
+                    t.work_start[i][b] = w[i];
+                }
                 v[0] += s.n;
                 v[1] += n;
                 v[2] += s.rel;
                 v[3] += s.need - s.keep;
                 v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
                 v[5] += (n + kKv8Block - 1) / kKv8Block;
-                const int tl = (s.n * a.group + a.tile_rows - 1) / a.tile_rows;
-                nt += tl;
-                w += (long long)tl * ((n + kPageSize - 1) / kPageSize);
+                const int li = s.n * a.group >= a.long_min, tr = li ? kKv8Long : a.tile_rows;
+                const int tl = (s.n * a.group + tr - 1) / tr;
+                nt[li] += tl;
+                w[li] += (long long)tl * ((n + kPageSize - 1) / kPageSize);
             }
             if (threadIdx.x == 0) {
                 t.row_start[a.nseq] = tot[0];
@@ -224,9 +236,13 @@ __global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
                 t.take_start[a.nseq] = tot[3];
                 t.unit_start[a.nseq] = tot[4];
                 t.gblk_start[a.nseq] = tot[5];
-                t.tile_start[a.nseq] = tott;
-                t.work_start[a.nseq] = totw;
-                *t.meta = Kv8Meta{a.nseq, tot[0], tot[4], tot[5], 0, mp, tott, totw};
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    t.tile_start[i][a.nseq] = tott[i];
+                    t.work_start[i][a.nseq] = totw[i];
+                }
+                *t.meta = Kv8Meta{a.nseq, tot[0], tot[4], tot[5], 0, 0,
+                                  {{tott[0], totw[0], mp[0]}, {tott[1], totw[1], mp[1]}}};
             }
         }
     }
@@ -547,7 +563,8 @@ int create(fl_kv8* h) {
     h->group = c.heads / c.kv_heads;
     h->tile_rows = c.dtype == FL_F32 ? 8 : 16;
     cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device);
-    h->parts = h->sms * kv8_attention_occupancy(c.head_dim, c.type, c.dtype);
+    h->parts[0] = h->sms * kv8_attention_occupancy(c.head_dim, c.type, c.dtype);
+    h->parts[1] = h->sms * kv8_prefill_occupancy(c.head_dim, c.type, c.dtype);
     const size_t S = c.max_seqs, R = c.max_rows, kvb = (size_t)c.pages * c.kv_heads * kPageSize * c.head_dim;
     h->k.resize(c.layers);
     h->v.resize(c.layers);
@@ -571,13 +588,18 @@ int create(fl_kv8* h) {
     FL_CHECK(alloc(h, &t.unit_row, R, true));
     for (int** p : {&t.row_start, &t.kv_start, &t.take_start, &t.rel_start, &t.unit_start, &t.gblk_start, &t.ctx})
         FL_CHECK(alloc(h, p, S + 1, true));
-    FL_CHECK(alloc(h, &t.tile_start, S + 1, true));
-    FL_CHECK(alloc(h, &t.work_start, S + 1, true));
+    for (int i = 0; i < 2; i++) {
+        FL_CHECK(alloc(h, &t.tile_start[i], S + 1, true));
+        FL_CHECK(alloc(h, &t.work_start[i], S + 1, true));
+    }
     FL_CHECK(alloc(h, &t.meta, 1, true));
     // a part begins inside a tile at most, and ends inside one
-    FL_CHECK(alloc(h, &h->part, (size_t)2 * h->parts * h->tile_rows * c.head_dim, false));
-    FL_CHECK(alloc(h, &h->part_ml, (size_t)2 * h->parts * h->tile_rows, false));
-    FL_CHECK(alloc(h, &h->part_cnt, h->parts, true));
+    for (int i = 0; i < 2; i++) {
+        const size_t rows = (size_t)2 * h->parts[i] * (i ? kKv8Long : h->tile_rows);
+        FL_CHECK(alloc(h, &h->part[i], rows * c.head_dim, false));
+        FL_CHECK(alloc(h, &h->part_ml[i], rows, false));
+        FL_CHECK(alloc(h, &h->part_cnt[i], h->parts[i], true));
+    }
     kv8_reset_kernel<<<64, 256>>>(t, c.pages, c.max_seqs);
     FL_CHECK_CUDA(cudaGetLastError());
     FL_CHECK_CUDA(cudaDeviceSynchronize());
@@ -679,6 +701,7 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     a.max_rows = h->c.max_rows;
     a.group = h->group;
     a.tile_rows = h->tile_rows;
+    a.long_min = kLongMin;
     // one CTA while its threads hold the rows; eight (a portable cluster) beyond
     const long long rows = std::min<long long>((long long)nseq * a.max_new, h->c.max_rows);
     cudaLaunchConfig_t cfg = {};
@@ -788,9 +811,10 @@ FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, in
     p.scale = scale * 1.4426950408889634f;
     p.mask = mask;
     p.ldm = ldm;
-    p.part = h->part;
-    p.part_ml = h->part_ml;
-    p.part_cnt = h->part_cnt;
-    FL_CHECK_CUDA(launch_kv8_attention(p, h->parts, s));
+    Kv8Tiles tl[2];
+    for (int i = 0; i < 2; i++)
+        tl[i] = Kv8Tiles{i, h->t.tile_start[i], h->t.work_start[i], h->part[i], h->part_ml[i], h->part_cnt[i]};
+    FL_CHECK_CUDA(launch_kv8_attention(p, tl[0], h->parts[0], s));
+    if ((long long)h->max_new * h->group >= kLongMin) FL_CHECK_CUDA(launch_kv8_prefill(p, tl[1], h->parts[1], s));
     return FL_OK;
 }

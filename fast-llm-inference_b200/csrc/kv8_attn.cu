@@ -22,6 +22,7 @@
 
 #include "fl_common.cuh"
 #include "fl_kv8.h"
+#include "fl_kv8_attn.cuh"
 #include "fl_kv8_types.cuh"
 
 namespace fl {
@@ -30,37 +31,11 @@ namespace {
 
 constexpr int kAW = 4;   // warps per CTA: one per 16-position block of a page
 constexpr int kStages = 4;   // blocks in flight or in use per warp
-constexpr float kTileCost = 3.0f, kJoinCost = 20.0f;   // in pages, see the kernel
-constexpr float kShift = 7.0f;   // probabilities enter as 2^7 p: 2^-21 of the largest is a normal half
-constexpr float kSlack = 8.0f;   // the reference follows the maximum once it lags by 2^8
-
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Four codes of a word as two half pairs.
-template <bool E4M3>
-__device__ __forceinline__ void codes_to_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if constexpr (E4M3) {
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-            : "=r"(lo), "=r"(hi)
-            : "r"(w));
-    } else {
-        const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
-        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-        lo = *reinterpret_cast<const uint32_t*>(&x);
-        hi = *reinterpret_cast<const uint32_t*>(&y);
-    }
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -80,99 +55,8 @@ __device__ __forceinline__ float2 lds8(uint32_t a) {
     return v;
 }
 
-// 8 values at dimensions d .. d + 7 of a query row.
-template <int DT>
-__device__ __forceinline__ void load8(const void* q, size_t i, int vec, float (&f)[8]) {
-    float a[4], b[4];
-    load4<DT>(q, i, vec, a);
-    load4<DT>(q, i + 4, vec, b);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        f[j] = a[j];
-        f[4 + j] = b[j];
-    }
-}
-
-// A range of a tile's pages.
-struct Kv8Item {
-    int seq, head, ctx, row0, nb;
-    int tile, page0, pages;   // no pages: none is left
-    int split, splits;        // this range among the tile's
-    int part;                 // the part that holds the tile's first page
-    long long next;           // where the CTA goes on
-};
-
-// The sequence whose work x falls into: start[b] <= x < start[b + 1]. A warp
-// narrows the range 32-fold a step.
-__device__ __forceinline__ int find_work(const long long* start, int nseq, long long x, int lane) {
-    int lo = 0, n = nseq;   // start[lo] <= x < start[lo + n]
-    while (n > 1) {
-        const int step = (n + 31) / 32;
-        const int at = lo + lane * step;
-        const bool below = lane * step < n && start[at] <= x;
-        const int k = 31 - __clz((int)__ballot_sync(0xffffffffu, below));
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    return lo;
-}
-
-// The work of a CTA, item by item (x: where it stands, -1 at first); by a warp.
-// Two ways to share it. Whole tiles, CTA by CTA; or the (kv head, row tile,
-// page) triples, in that order, cut into equal parts, one a CTA, which end
-// together whatever the lengths are, while a tile that several parts share is
-// joined by the last of them to arrive. What each takes is estimated in pages:
-// kTileCost a tile, kJoinCost for the joins. At 64 x 32 tiles of 21 pages whole
-// tiles took 106 us and parts 120; at 24 x 10 tiles of 5 to 500, 290 and 168.
-__device__ __forceinline__ void next_item(const Kv8AttnParams& p, long long x, int lane, Kv8Item& out) {
-    const Kv8Meta& mt = *p.t.meta;
-    const long long tiles = mt.tiles, work = mt.work, G = gridDim.x;
-    const float mean = (float)work / (float)max(1ll, tiles), per_cta = (float)(tiles * p.kv_heads) / (float)G;
-    const bool whole = ceilf(per_cta) * (mean + kTileCost) + ((float)mt.max_pages - mean) <=
-                       per_cta * mean + (per_cta + 1.0f) * kTileCost + kJoinCost;
-    const long long total = (whole ? tiles : work) * p.kv_heads;
-    const long long size = whole ? 1 : (total + G - 1) / G;
-    if (x < 0) x = (long long)blockIdx.x * size;
-    Kv8Item it = {};
-    if (x < (whole ? total : min(total, (blockIdx.x + 1ll) * size))) {
-        it.head = (int)(x / (whole ? tiles : work));
-        const long long in_head = x - it.head * (whole ? tiles : work);
-        const long long* start = whole ? p.t.tile_start : p.t.work_start;
-        it.seq = find_work(start, mt.seqs, in_head, lane);
-        const long long in_seq = in_head - start[it.seq];
-        it.ctx = p.t.ctx[it.seq];
-        it.row0 = p.t.row_start[it.seq];
-        it.nb = p.t.row_start[it.seq + 1] - it.row0;
-        it.pages = (it.ctx + it.nb + kPageSize - 1) / kPageSize;
-        it.splits = 1;
-        if (whole) {
-            it.tile = (int)in_seq;
-            it.next = x + G;
-        } else {
-            const int tile_pages = it.pages;
-            it.tile = (int)(in_seq / tile_pages);
-            it.page0 = (int)(in_seq - (long long)it.tile * tile_pages);
-            it.pages = (int)min((long long)(tile_pages - it.page0), (blockIdx.x + 1ll) * size - x);
-            const long long tile_x = x - it.page0;   // the tile's first triple
-            it.part = (int)(tile_x / size);
-            it.splits = (int)((tile_x + tile_pages - 1) / size) - it.part + 1;
-            it.split = (int)blockIdx.x - it.part;
-            it.next = x + it.pages;
-        }
-    }
-    if (lane == 0) out = it;
-}
-
-// Shift of a row with largest magnitude a: a 2^sh in [2^14, 2^15); 0 for a
-// zero row and for one that is not finite (its results are NaN).
-__device__ __forceinline__ float row_shift(float a) {
-    const int x = (int)((__float_as_uint(a) >> 23) & 255u);
-    if (x == 0 || x == 255) return 1.0f;
-    return __uint_as_float((uint32_t)min(max(127 + 14 - (x - 127), 1), 253) << 23);
-}
-
 template <int HD, int DT, bool E4M3>
-__global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8AttnParams p, const int vec) {
+__global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8AttnParams p, const Kv8Tiles tl, const int vec) {
     constexpr bool F32 = DT == FL_F32;
     constexpr int TR = F32 ? 8 : 16;   // query rows per tile
     constexpr int NC = HD / 32;
@@ -187,7 +71,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
     const int g = lane >> 2, t4 = lane & 3;
     __shared__ Kv8Item it;   // re-read where it is used: registers go to the tile
     for (long long x = -1;;) {
-        if (warp == 0) next_item(p, x, lane, it);
+        if (warp == 0) next_item(p, tl, x, lane, it);
         __syncthreads();
         if (it.pages == 0) break;
         x = it.next;
@@ -356,7 +240,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
 #pragma unroll
                 for (int r = 0; r < RR; r++) {
                     const float mn = fmaxf(m[r], mx[r]);
-                    const float al = m[r] == -INFINITY ? 0.0f : exp2f(m[r] - mn);
+                    const float al = m[r] == -INFINITY ? 0.0f : ex2(m[r] - mn);
                     m[r] = mn;
                     l[r] *= al;
                     const float f = al * vr;
@@ -381,7 +265,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                 float pr[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    pr[e] = exp2f(s[r][e] - mr);
+                    pr[e] = ex2(s[r][e] - mr);
                     l[r] += pr[e];
                     pr[e] *= vf;
                 }
@@ -442,7 +326,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
 #pragma unroll
             for (int k = 0; k < kAW; k++) {
                 if (l_s[k][r] == 0.0f) continue;
-                const float wk = l_s[k][r] * exp2f(m_s[k][r] - M);
+                const float wk = l_s[k][r] * ex2(m_s[k][r] - M);
                 L += wk;
                 const float4 v = *reinterpret_cast<const float4*>(&o_s[k][r][d]);
                 acc[0] += wk * v.x; acc[1] += wk * v.y; acc[2] += wk * v.z; acc[3] += wk * v.w;
@@ -451,8 +335,8 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[j] *= f;
             if (it.splits > 1) {
-                *reinterpret_cast<float4*>(p.part + (slot * TR + r) * HD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                if (d == 0) p.part_ml[slot * TR + r] = make_float2(M, L);
+                *reinterpret_cast<float4*>(tl.part + (slot * TR + r) * HD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                if (d == 0) tl.part_ml[slot * TR + r] = make_float2(M, L);
             } else {
                 const int pr = it.tile * TR + r, tk = pr / p.group;
                 const int hq = h * p.group + pr - tk * p.group;
@@ -461,7 +345,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
         }
         if (it.splits > 1) {
             // the last range to arrive joins the tile's ranges, in their order
-            int* cnt = p.part_cnt + it.part;
+            int* cnt = tl.part_cnt + it.part;
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) last_s = atomicAdd(cnt, 1) == it.splits - 1;
@@ -470,22 +354,8 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                 __threadfence();
                 for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kAW * 32) {
                     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
-                    float M = -INFINITY;
-                    for (int k = 0; k < it.splits; k++)
-                        M = fmaxf(M, __ldcg(&p.part_ml[(2 * (size_t)(it.part + k) + (k == 0)) * TR + r]).x);
-                    float L = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-                    for (int k = 0; k < it.splits; k++) {
-                        const size_t sk = (2 * (size_t)(it.part + k) + (k == 0)) * TR + r;
-                        const float2 ml = __ldcg(&p.part_ml[sk]);
-                        if (ml.y == 0.0f) continue;
-                        const float wk = ml.y * exp2f(ml.x - M);
-                        L += wk;
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + sk * HD + d));
-                        acc[0] += wk * v.x; acc[1] += wk * v.y; acc[2] += wk * v.z; acc[3] += wk * v.w;
-                    }
-                    const float f = L != 0.0f ? __fdiv_rn(1.0f, L) : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[j] *= f;
+                    float acc[4];
+                    join_parts(tl, it, TR, HD, r, d, acc);
                     const int pr = it.tile * TR + r, tk = pr / p.group;
                     const int hq = h * p.group + pr - tk * p.group;
                     if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
@@ -537,12 +407,12 @@ int kv8_attention_occupancy(int head_dim, int type, int dtype) {
     return n > 0 ? n : 1;
 }
 
-cudaError_t launch_kv8_attention(const Kv8AttnParams& p, int ctas, cudaStream_t s) {
+cudaError_t launch_kv8_attention(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s) {
     const int es = p.dtype == FL_F32 ? 4 : 2;
     const int vec = ((uintptr_t)p.q & 15) == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldq * es % 16 == 0 &&
                     p.ldo * es % 16 == 0;
     return with_kernel(p.head_dim, p.type, p.dtype, [&](auto* k) {
-        k<<<ctas, kAW * 32, attention_smem(p.head_dim, p.dtype), s>>>(p, vec);
+        k<<<ctas, kAW * 32, attention_smem(p.head_dim, p.dtype), s>>>(p, tl, vec);
         return cudaGetLastError();
     });
 }

@@ -1,0 +1,631 @@
+// Attention of many query rows over the paged 8-bit KV cache (prompt chunks,
+// draft trees of grouped heads) on the 5th-generation tensor cores, sm_100a.
+// The mathematics is that of kv8_attn.cu.
+//
+// A tile is 128 packed query rows of one kv head against pages of 64 keys:
+// S = Q K^T (128 x 64) and O += P V (128 x head_dim), both tcgen05.mma.kind::f16
+// with operands in shared memory (SWIZZLE_128B, K-major) and accumulators in
+// TMEM: two S buffers of 64 columns, O behind them.
+//  - warps 0-3: softmax, one query row a thread. They write Q at first, then per
+//    page read S (tcgen05.ld), keep the running reference and sum, and write P as
+//    halves. The reference follows the maximum only once it lags by 2^8, so O is
+//    seldom read back and rescaled.
+//  - warps 4-7: conversion, one 16-position block of the page a warp. The codes
+//    come as 16-byte pieces (fl_kv8.h), a page ahead of their use, and go to shared
+//    memory as halves: a K piece is two 16-byte chunks of two keys' rows; a V piece
+//    holds four keys of four dimensions, so V^T is written without a transposition.
+//    V is scaled by its block's scale over the largest so far (a power of two, in
+//    the multiply-add that removes the INT8 offset).
+//  - warp 8: one thread issues the products: S of the next page before P V of this.
+// Two CTAs share an SM (112 KB and 256 TMEM columns each at most for 16-bit rows),
+// so that one's softmax runs beside the other's products. f32 rows take two halves
+// for Q and for P (22 bits): twice the products, and one CTA per SM.
+//
+// Bound by issue: per page and tile about 2600 warp instructions of softmax and
+// 1000 of conversion against 511 cycles of products.
+//
+// Waits are bounded (2 s of %globaltimer); on expiry the CTA raises an error word,
+// stops, waits (bounded) for its own products, frees TMEM and exits.
+#include <math.h>
+
+#include <algorithm>
+
+#include "fl_common.cuh"
+#include "fl_kv8.h"
+#include "fl_kv8_attn.cuh"
+#include "fl_kv8_types.cuh"
+
+namespace fl {
+
+namespace {
+
+__device__ int g_kv8_error = 0;
+
+constexpr int kRows = kKv8Long;          // query rows of a tile
+constexpr int kThreads = 9 * 32;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr float kVUp = 32.0f;            // V enters as 2^5 code / largest scale: 1152 2^5, the offset, is a half
+
+__device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mb_init(uint64_t* b, uint32_t n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mb_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(b)) : "memory");
+}
+__device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t par) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(saddr(b)), "r"(par)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ unsigned long long gtime() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+__device__ __noinline__ bool mb_wait_slow(uint64_t* b, uint32_t par) {
+    const unsigned long long t0 = gtime();
+    while (!mb_try(b, par))
+        if (gtime() - t0 > kWaitNs) {
+            atomicOr(&g_kv8_error, 1);
+            return false;
+        }
+    return true;
+}
+__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t par) { return mb_try(b, par) || mb_wait_slow(b, par); }
+
+// By a whole warp: one lane waits.
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t par) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mb_wait(b, par) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// The largest V scale of a page's blocks that hold positions below end.
+__device__ __forceinline__ float vscale_max(const float4& v, int k0, int end) {
+    float m = k0 < end ? v.x : 0.0f;
+    if (k0 + kKv8Block < end) m = fmaxf(m, v.y);
+    if (k0 + 2 * kKv8Block < end) m = fmaxf(m, v.z);
+    if (k0 + 3 * kKv8Block < end) m = fmaxf(m, v.w);
+    return m;
+}
+
+// A page's scales, loaded a page ahead of their use (and its number two ahead).
+struct Scales {
+    float4 k, v;
+    int page;   // of the page after the loaded one
+    __device__ __forceinline__ Scales(const Kv8AttnParams& p, const int* bt, int h, int n) : page(0) {
+        k = v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (n > 0) page = bt[0];
+        load(p, bt, h, 0, n);
+    }
+    __device__ __forceinline__ void load(const Kv8AttnParams& p, const int* bt, int h, int j, int n) {
+        if (j >= n) return;
+        const size_t at = ((size_t)page * p.kv_heads + h) * kKv8Sub;
+        k = *reinterpret_cast<const float4*>(p.ks + at);
+        v = *reinterpret_cast<const float4*>(p.vs + at);
+        if (j + 1 < n) page = bt[j + 1];
+    }
+};
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {   // 128-byte swizzled K-major rows, 8-row groups
+    uint64_t d = (uint64_t)((addr >> 4) & 0x3FFF);
+    d |= (uint64_t)(16 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// D (f32, TMEM) (+)= A (f16, 128 x 16) B (f16, N x 16)^T.
+template <int N>
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, bool acc) {
+    constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(b))
+                 : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t ta, float* f) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(ta));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t ta, const float* f) {
+    const uint32_t* v = reinterpret_cast<const uint32_t*>(f);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(ta),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void sts8(uint32_t a, uint32_t x, uint32_t y) {
+    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+
+// Four V codes of a word as two half pairs times r (a power of two; off = -1152 r).
+template <bool E4M3>
+__device__ __forceinline__ void scaled_halves(uint32_t w, __half2 r, __half2 off, uint32_t& lo, uint32_t& hi) {
+    if constexpr (E4M3) {
+        uint32_t a, b;
+        codes_to_halves<true>(w, a, b);
+        const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), r);
+        const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&b), r);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&a), r, off);
+        const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), r, off);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
+// Shared memory of a CTA, in bytes from a 1024-byte boundary.
+template <int HD, bool F32>
+struct Layout {
+    static constexpr int kCb = (HD + 63) / 64;                 // 64-dimension column blocks
+    static constexpr int kParts = F32 ? 2 : 1;                 // halves per value of Q and P
+    static constexpr int kQ = 0, kQPart = kCb * kRows * 128;
+    static constexpr int kK = kQ + kParts * kQPart;
+    static constexpr int kV = kK + kCb * kPageSize * 128;
+    static constexpr int kP = kV + HD * 128, kPPart = kRows * 128;
+    static constexpr int kBytes = kP + kParts * kPPart + 1024;
+};
+
+template <int HD, int DT, bool E4M3>
+__global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
+    kv8_prefill_kernel(const Kv8AttnParams p, const Kv8Tiles tl, const int vec) {
+    constexpr bool F32 = DT == FL_F32;
+    typedef Layout<HD, F32> L;
+    constexpr int NC = HD / 32;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t k_full, k_empty, v_full, pv_done, p_full, s_full[2], s_empty[2];
+    __shared__ uint32_t tmem_s;
+    __shared__ int bad_s, last_s;
+    __shared__ Kv8Item it;
+    const uint32_t smem = (saddr(smem_raw) + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mb_init(&k_full, 4);
+        mb_init(&k_empty, 1);
+        mb_init(&v_full, 4);
+        mb_init(&pv_done, 1);
+        mb_init(&p_full, 4);
+        for (int i = 0; i < 2; i++) {
+            mb_init(&s_full[i], 1);
+            mb_init(&s_empty[i], 4);
+        }
+        bad_s = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(saddr(&tmem_s)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = tmem_s;
+    uint32_t J0 = 0;   // pages of the items before: the phases of the barriers run on
+
+    for (long long x = -1;;) {
+        if (warp == 0) next_item(p, tl, x, lane, it);
+        __syncthreads();
+        if (it.pages == 0 || bad_s) break;
+        x = it.next;
+        const int h = it.head, ctx = it.ctx, row0 = it.row0, nb = it.nb;
+        const int np = min(kRows, nb * p.group - it.tile * kRows);
+        const int tok_last = (it.tile * kRows + np - 1) / p.group;
+        const int kend = p.mask ? ctx + nb : ctx + tok_last + 1;
+        const int k0 = it.page0 * kPageSize;                 // first key of the range
+        const int n = max(0, min(it.pages, (kend - k0 + kPageSize - 1) / kPageSize));
+        const int* bt = p.t.block_table + (size_t)it.seq * p.max_pages + it.page0;
+
+        if (warp < 4) {
+            // ------------------------------------------------------- softmax
+            const int r = threadIdx.x;
+            const int pr = it.tile * kRows + r, tok = pr / p.group;
+            const int head = h * p.group + pr - tok * p.group, row = row0 + tok;
+            const bool live = r < np && row < p.rows;
+            const size_t qat = (size_t)row * p.ldq + (size_t)head * HD;
+            float amax = 0.0f;
+            if (live) {
+#pragma unroll 4
+                for (int c = 0; c < HD / 4; c++) {
+                    float f[4];
+                    load4<DT>(p.q, qat + 4 * c, vec, f);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) amax = fmaxf(amax, fabsf(f[j]));
+                }
+            }
+            // |scale| goes to the scores, its sign to the queries: factors stay positive
+            const float sh = row_shift(amax);
+            const float unshift = pow2_inv(sh) * fabsf(p.scale), qs = p.scale < 0.0f ? -sh : sh;
+#pragma unroll 2
+            for (int c = 0; c < HD / 8; c++) {
+                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (live) load8<DT>(p.q, qat + 8 * c, vec, f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] *= qs;
+                const uint32_t a = smem + L::kQ + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                sts16(a, h2(f[0], f[1]), h2(f[2], f[3]), h2(f[4], f[5]), h2(f[6], f[7]));
+                if constexpr (F32) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) f[j] -= __half2float(__float2half_rn(f[j]));
+                    sts16(a + L::kQPart, h2(f[0], f[1]), h2(f[2], f[3]), h2(f[4], f[5]), h2(f[6], f[7]));
+                }
+            }
+            proxy_fence();
+            __syncwarp();
+            bool ok = true;
+            // Q is there and both S buffers are free: s_empty grants pages J0 and J0 + 1
+            if (lane == 0 && n > 0) mb_arrive(&s_empty[J0 & 1]);
+            if (lane == 0 && n > 1) mb_arrive(&s_empty[(J0 + 1) & 1]);
+            const uint32_t tq = tmem + ((uint32_t)(32 * warp) << 16);
+            float m = -INFINITY, l = 0.0f, vref = 0.0f;
+            const int lim = p.mask ? ctx + nb : ctx + tok + 1;   // positions this row may see
+            const uint8_t* mrow = p.mask && live ? p.mask + (size_t)row * p.ldm : nullptr;
+            Scales next(p, bt, h, n);
+            for (int j = 0; j < n; j++) {
+                const uint32_t J = J0 + j;
+                const float4 ks4 = next.k;
+                const float vs = vscale_max(next.v, k0 + j * kPageSize, ctx + nb);
+                next.load(p, bt, h, j + 1, n);
+                if (!warp_wait(&s_full[J & 1], (J >> 1) & 1)) { ok = false; break; }
+                tc_after();
+                // S twice, 32 columns at a time: 64 values would not stay in registers
+                const uint32_t sb = tq + (J & 1) * 64;
+                const float f[4] = {ks4.x * unshift, ks4.y * unshift, ks4.z * unshift, ks4.w * unshift};
+                const int kb = k0 + j * kPageSize;
+                const bool part = kb + kPageSize > ctx + (p.mask ? 0 : it.tile * kRows / p.group);
+                // bit i: this row sees column i
+                uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+                if (part) {
+                    const int left = lim - kb;
+                    see[0] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+                    see[1] = left >= 64 ? 0xffffffffu : left <= 32 ? 0u : (1u << (left - 32)) - 1u;
+                    if (p.mask) {
+                        unsigned long long hide = 0;
+                        for (int i = max(0, ctx - kb); i < min(64, left); i++)
+                            if (!mrow || mrow[kb + i - ctx] == 0) hide |= 1ull << i;
+                        see[0] &= ~(uint32_t)hide;
+                        see[1] &= ~(uint32_t)(hide >> 32);
+                    }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    float s[32];
+                    tmem_ld32(sb + 32 * w, s);
+                    tmem_wait_ld();
+                    if (part) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            mx = fmaxf(mx, (see[w] >> i) & 1 ? s[i] * f[2 * w + (i >> 4)] : -INFINITY);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            float bm = s[16 * b];
+#pragma unroll
+                            for (int i = 1; i < 16; i++) bm = fmaxf(bm, s[16 * b + i]);
+                            mx = fmaxf(mx, bm * f[2 * w + b]);
+                        }
+                    }
+                }
+                // P's buffer, and O: the products of the page before have to be done
+                if (j > 0 && !warp_wait(&pv_done, (J - 1) & 1)) { ok = false; break; }
+                const float vnew = fmaxf(vref, vs);
+                const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
+                if (j == 0) {
+                    m = mx;
+                } else if (__any_sync(0xffffffffu, move || vnew > vref)) {
+                    const float mn = fmaxf(m, mx);
+                    const float al = m == -INFINITY ? 0.0f : ex2(m - mn);
+                    m = mn;
+                    l *= al;
+                    const float g = al * (vref * pow2_inv(vnew));
+                    tc_after();
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        float o[32];
+                        tmem_ld32(tq + 128 + 32 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] *= g;
+                        tmem_st32(tq + 128 + 32 * c, o);
+                    }
+                    tmem_wait_st();
+                }
+                vref = vnew;
+                const float mr = m == -INFINITY ? 0.0f : m - kShift;
+                const uint32_t pa = smem + L::kP + r * 128;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    float s[32];
+                    tmem_ld32(sb + 32 * w, s);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float e[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            e[i] = ex2(__fmaf_rn(s[8 * c + i], f[2 * w + (c >> 1)], -mr));
+                            if (part && !((see[w] >> (8 * c + i)) & 1)) e[i] = 0.0f;
+                            l += e[i];
+                        }
+                        const uint32_t a = pa + (((4 * w + c) ^ (r & 7)) << 4);
+                        sts16(a, h2(e[0], e[1]), h2(e[2], e[3]), h2(e[4], e[5]), h2(e[6], e[7]));
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) e[i] -= __half2float(__float2half_rn(e[i]));
+                            sts16(a + L::kPPart, h2(e[0], e[1]), h2(e[2], e[3]), h2(e[4], e[5]), h2(e[6], e[7]));
+                        }
+                    }
+                }
+                tc_before();
+                __syncwarp();
+                if (lane == 0 && j + 2 < n) mb_arrive(&s_empty[J & 1]);   // S is read: free for page J + 2
+                proxy_fence();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&p_full);
+            }
+            // the row's output: normalised, to its place or to the part's slot
+            if (ok && n > 0) ok = warp_wait(&pv_done, (J0 + n - 1) & 1);
+            if (!ok) {
+                if (lane == 0) atomicOr(&bad_s, 1);
+            } else {
+                tc_after();
+                const size_t slot = 2 * (size_t)blockIdx.x + (it.split == 0);
+                const float g = l != 0.0f ? __fdiv_rn(vref * (1.0f / kVUp), l) : 0.0f;
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    float o[32];
+                    if (n > 0) {
+                        tmem_ld32(tq + 128 + 32 * c, o);
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float v[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) v[k] = n > 0 && l != 0.0f ? o[i + k] * g : 0.0f;
+                        if (it.splits > 1)
+                            *reinterpret_cast<float4*>(tl.part + (slot * kRows + r) * HD + c * 32 + i) =
+                                make_float4(v[0], v[1], v[2], v[3]);
+                        else if (live)
+                            store4<DT>(p.out, (size_t)row * p.ldo + (size_t)head * HD + c * 32 + i, vec, v);
+                    }
+                }
+                if (it.splits > 1) tl.part_ml[slot * kRows + r] = make_float2(m, l);
+                tc_before();
+            }
+        } else if (warp < 8) {
+            // ---------------------------------------------------- conversion
+            const int blk = warp - 4, t4 = lane & 3, g = lane >> 2;
+            // the next page's K codes are loaded once this page's are converted, and
+            // its V codes likewise; page numbers and scales a page ahead
+            uint4 kq[NC], vq[NC];
+            Scales next(p, bt, h, n);
+            size_t off = 0;
+            auto load_k = [&](int page) {
+                off = ((size_t)page * p.kv_heads + h) * (kPageSize * HD) + blk * (kKv8Block * HD) + lane * 16;
+#pragma unroll
+                for (int c = 0; c < NC; c++) kq[c] = ld_stream16(p.k + off + c * 512);
+            };
+            auto load_v = [&]() {
+#pragma unroll
+                for (int c = 0; c < NC; c++) vq[c] = ld_stream16(p.v + off + c * 512);
+            };
+            float vref = 0.0f;
+            bool ok = true;
+            if (n > 0) {
+                load_k(bt[0]);
+                load_v();
+            }
+            for (int j = 0; j < n; j++) {
+                const uint32_t J = J0 + j;
+                const float4 vs4 = next.v;
+                const int after = next.page;   // of page j + 1
+                next.load(p, bt, h, j + 1, n);
+                const int kb = k0 + j * kPageSize + blk * kKv8Block;
+                vref = fmaxf(vref, vscale_max(vs4, k0 + j * kPageSize, ctx + nb));
+                const float vs = blk < 2 ? (blk ? vs4.y : vs4.x) : (blk == 2 ? vs4.z : vs4.w);
+                const float ratio = kb < ctx + nb ? vs * pow2_inv(vref) * kVUp : 0.0f;
+                if (J > 0 && !warp_wait(&k_empty, (J - 1) & 1)) { ok = false; break; }
+                // K rows: key 16 blk + 4 (g / 2) + (g & 1) + 2 half, dimensions 32 c + 8 t4 .. + 7
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const uint32_t w[4] = {kq[c].x, kq[c].y, kq[c].z, kq[c].w};
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        uint32_t a, b, d, e;
+                        codes_to_halves<E4M3>(w[2 * half], a, b);
+                        codes_to_halves<E4M3>(w[2 * half + 1], d, e);
+                        const int key = blk * kKv8Block + 4 * (g >> 1) + (g & 1) + 2 * half;
+                        sts16(smem + L::kK + (c >> 1) * (kPageSize * 128) + key * 128 +
+                                  (((((c & 1) << 2) + t4) ^ (key & 7)) << 4), a, b, d, e);
+                    }
+                }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&k_full);
+                if (j + 1 < n) load_k(after);
+                if (J > 0 && !warp_wait(&pv_done, (J - 1) & 1)) { ok = false; break; }
+                // V^T rows: dimension 32 c + 4 g + i, keys 16 blk + 4 t4 .. + 3; positions
+                // behind the sequence may hold anything, an E4M3 NaN too
+                const int left = ctx + nb - kb - 4 * t4;
+                const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+                const __half2 rr = __floats2half2_rn(ratio, ratio), off = __floats2half2_rn(-1152.0f * ratio, -1152.0f * ratio);
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const uint32_t w[4] = {vq[c].x, vq[c].y, vq[c].z, vq[c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t a, b;
+                        scaled_halves<E4M3>(E4M3 ? w[i] & keep : w[i], rr, off, a, b);
+                        const int d = c * 32 + 4 * g + i;
+                        sts8(smem + L::kV + d * 128 + (((2 * blk + (t4 >> 1)) ^ (d & 7)) << 4) + (t4 & 1) * 8, a, b);
+                    }
+                }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mb_arrive(&v_full);
+                if (j + 1 < n) load_v();
+            }
+            if (!ok && lane == 0) atomicOr(&bad_s, 1);
+        } else if (lane == 0) {
+            // ------------------------------------------------------ products
+            bool ok = true;
+            uint32_t nqk = J0, npv = J0;   // pages whose products are issued
+            auto scores = [&](uint32_t J) -> bool {   // S of page J into buffer J & 1
+                if (!mb_wait(&s_empty[J & 1], (J >> 1) & 1) || !mb_wait(&k_full, J & 1)) return false;
+                tc_after();
+#pragma unroll
+                for (int q = 0; q < L::kParts; q++)
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++)
+                        umma_f16<kPageSize>(tmem + (J & 1) * 64,
+                                            desc_sw128(smem + L::kQ + q * L::kQPart + (k >> 2) * (kRows * 128) + (k & 3) * 32),
+                                            desc_sw128(smem + L::kK + (k >> 2) * (kPageSize * 128) + (k & 3) * 32),
+                                            q + k > 0);
+                umma_commit(&k_empty);
+                umma_commit(&s_full[J & 1]);
+                nqk = J + 1;
+                return true;
+            };
+            if (n > 0) ok = scores(J0);
+            for (int j = 0; j < n && ok; j++) {
+                const uint32_t J = J0 + j;
+                if (j + 1 < n && !scores(J + 1)) { ok = false; break; }
+                if (!mb_wait(&p_full, J & 1) || !mb_wait(&v_full, J & 1)) { ok = false; break; }
+                tc_after();
+#pragma unroll
+                for (int q = 0; q < L::kParts; q++)
+#pragma unroll
+                    for (int k = 0; k < kPageSize / 16; k++)
+                        umma_f16<HD>(tmem + 128, desc_sw128(smem + L::kP + q * L::kPPart + k * 32),
+                                     desc_sw128(smem + L::kV + k * 32), j > 0 || q + k > 0);
+                umma_commit(&pv_done);
+                npv = J + 1;
+            }
+            if (!ok) {   // the products under way read this CTA's memory: wait for them, too
+                if (nqk > J0) (void)mb_wait(&k_empty, (nqk - 1) & 1);
+                if (npv > J0) (void)mb_wait(&pv_done, (npv - 1) & 1);
+                atomicOr(&bad_s, 1);
+            }
+        }
+        __syncthreads();
+        if (bad_s) break;
+        J0 += n;
+        if (it.splits > 1) {
+            // the last range to arrive joins the tile's ranges, in their order
+            int* cnt = tl.part_cnt + it.part;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) last_s = atomicAdd(cnt, 1) == it.splits - 1;
+            __syncthreads();
+            if (last_s) {
+                __threadfence();
+                for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kThreads) {
+                    const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+                    float acc[4];
+                    join_parts(tl, it, kRows, HD, r, d, acc);
+                    const int pr = it.tile * kRows + r, tk = pr / p.group;
+                    const int hq = h * p.group + pr - tk * p.group;
+                    if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
+                }
+                if (threadIdx.x == 0) *cnt = 0;
+            }
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+    }
+}
+
+template <class F>
+cudaError_t with_kernel(int hd, int type, int dtype, F f) {
+#define FL_KV8_K(HD)                                                                                            \
+    if (hd == HD) {                                                                                             \
+        if (type == FL_KV8_E4M3)                                                                                \
+            return dtype == FL_F32   ? f(kv8_prefill_kernel<HD, FL_F32, true>, Layout<HD, true>::kBytes)        \
+                   : dtype == FL_F16 ? f(kv8_prefill_kernel<HD, FL_F16, true>, Layout<HD, false>::kBytes)       \
+                                     : f(kv8_prefill_kernel<HD, FL_BF16, true>, Layout<HD, false>::kBytes);     \
+        return dtype == FL_F32   ? f(kv8_prefill_kernel<HD, FL_F32, false>, Layout<HD, true>::kBytes)           \
+               : dtype == FL_F16 ? f(kv8_prefill_kernel<HD, FL_F16, false>, Layout<HD, false>::kBytes)          \
+                                 : f(kv8_prefill_kernel<HD, FL_BF16, false>, Layout<HD, false>::kBytes);        \
+    }
+    FL_KV8_K(32)
+    FL_KV8_K(64)
+    FL_KV8_K(96)
+    FL_KV8_K(128)
+#undef FL_KV8_K
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+int kv8_prefill_occupancy(int head_dim, int type, int dtype) {
+    int n = 0;
+    with_kernel(head_dim, type, dtype, [&](auto* k, int smem) {
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, smem);
+        return e;
+    });
+    return std::min(std::max(n, 1), 2);   // TMEM: 256 of 512 columns each
+}
+
+cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s) {
+    const int es = p.dtype == FL_F32 ? 4 : 2;
+    const int vec = ((uintptr_t)p.q & 15) == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldq * es % 16 == 0 &&
+                    p.ldo * es % 16 == 0;
+    return with_kernel(p.head_dim, p.type, p.dtype, [&](auto* k, int smem) {
+        k<<<ctas, kThreads, smem, s>>>(p, tl, vec);
+        return cudaGetLastError();
+    });
+}
+
+int take_kv8_error() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_kv8_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) {
+        const int z = 0;
+        cudaMemcpyToSymbol(g_kv8_error, &z, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace fl

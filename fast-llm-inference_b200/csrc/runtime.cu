@@ -10,6 +10,7 @@
 
 #include "fl_common.cuh"
 #include "fl_kernels.h"
+#include "fl_kv8.h"
 #include "fl_layout.cuh"
 #include "fl_runtime.h"
 
@@ -271,7 +272,7 @@ FL_API int fl_cuda_sync(void) {
     cudaStream_t s = device_stream();
     if (!s) return set_error(FL_E_NODEV, "no device");
     FL_CHECK_CUDA(cudaStreamSynchronize(s));
-    if (take_device_error() != 0) return set_error(FL_E_TIMEOUT, "a bounded device-side wait gave up");
+    if ((take_device_error() | take_kv8_error()) != 0) return set_error(FL_E_TIMEOUT, "a bounded device-side wait gave up");
     return FL_OK;
 }
 
