@@ -15,7 +15,7 @@ namespace fl {
 
 constexpr int kKv8Block = FL_KV8_BLOCK;           // positions per scale
 constexpr int kKv8Sub = kPageSize / kKv8Block;    // scales per page and head
-constexpr int kKv8Long = 128;                     // packed query rows of a tile of the prefill kernel
+constexpr int kKv8Long = 256;                     // packed query rows that a CTA of the prefill kernel takes
 
 // Codes of one (page, kv head) are kPageSize * head_dim bytes: per block of
 // 16 positions, per chunk of 32 dimensions, 512 bytes in the order in which a
@@ -106,7 +106,7 @@ cudaError_t launch_kv8_attention(const Kv8AttnParams& p, const Kv8Tiles& tl, int
 cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s);
 // CTAs of the attention kernel that one SM holds (for the plan's split).
 int kv8_attention_occupancy(int head_dim, int type, int dtype);
-int kv8_prefill_occupancy(int head_dim, int type, int dtype);
+cudaError_t kv8_prefill_prepare(int head_dim, int type, int dtype);
 int take_kv8_error();   // returns and clears the prefill kernel's error word
 
 }  // namespace fl

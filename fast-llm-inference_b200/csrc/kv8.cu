@@ -564,7 +564,8 @@ int create(fl_kv8* h) {
     h->tile_rows = c.dtype == FL_F32 ? 8 : 16;
     cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, h->device);
     h->parts[0] = h->sms * kv8_attention_occupancy(c.head_dim, c.type, c.dtype);
-    h->parts[1] = h->sms * kv8_prefill_occupancy(c.head_dim, c.type, c.dtype);
+    FL_CHECK_CUDA(kv8_prefill_prepare(c.head_dim, c.type, c.dtype));
+    h->parts[1] = h->sms;   // one CTA holds an SM's TMEM
     const size_t S = c.max_seqs, R = c.max_rows, kvb = (size_t)c.pages * c.kv_heads * kPageSize * c.head_dim;
     h->k.resize(c.layers);
     h->v.resize(c.layers);

@@ -2,29 +2,29 @@
 // draft trees of grouped heads) on the 5th-generation tensor cores, sm_100a.
 // The mathematics is that of kv8_attn.cu.
 //
-// A tile is 128 packed query rows of one kv head against pages of 64 keys:
-// S = Q K^T (128 x 64) and O += P V (128 x head_dim), both tcgen05.mma.kind::f16
-// with operands in shared memory (SWIZZLE_128B, K-major) and accumulators in
-// TMEM: two S buffers of 64 columns, O behind them.
-//  - warps 0-3: softmax, one query row a thread. They write Q at first, then per
-//    page read S (tcgen05.ld), keep the running reference and sum, and write P as
-//    halves. The reference follows the maximum only once it lags by 2^8, so O is
-//    seldom read back and rescaled.
-//  - warps 4-7: conversion, one 16-position block of the page a warp. The codes
-//    come as 16-byte pieces (fl_kv8.h), a page ahead of their use, and go to shared
-//    memory as halves: a K piece is two 16-byte chunks of two keys' rows; a V piece
-//    holds four keys of four dimensions, so V^T is written without a transposition.
-//    V is scaled by its block's scale over the largest so far (a power of two, in
-//    the multiply-add that removes the INT8 offset).
-//  - warp 8: one thread issues the products: S of the next page before P V of this.
-// Two CTAs share an SM (112 KB and 256 TMEM columns each at most for 16-bit rows),
-// so that one's softmax runs beside the other's products. f32 rows take two halves
-// for Q and for P (22 bits): twice the products, and one CTA per SM.
+// A CTA takes two tiles of 128 packed query rows of one kv head at a time,
+// against pages of 64 keys: S = Q K^T (128 x 64) and O += P V (128 x head_dim), all
+// tcgen05.mma.kind::f16, K, V and Q in shared memory (SWIZZLE_128B, K-major), P in
+// TMEM, accumulators in TMEM: per tile two S buffers of 64 columns and O, 512
+// columns in all.
+//  - warps 0-3 and 4-7: softmax of either tile, one query row a thread. They write
+//    Q at first, then per page read S (tcgen05.ld), keep the running reference and
+//    sum, and write P as halves over S (from shared memory, whose bandwidth bounds
+//    the products, P would be written and read once more). The reference follows the
+//    maximum only once it lags by 2^8, so O is seldom read back and rescaled.
+//  - warps 8-11: conversion, one 16-position block of the page a warp. The codes
+//    come as 16-byte pieces (fl_kv8.h), a page ahead of their use, and go to one of
+//    two stages as halves: a K piece is two 16-byte chunks of two keys' rows; a V
+//    piece holds four keys of four dimensions, so V^T is written without a
+//    transposition. V is scaled by its block's scale over the largest so far (a power
+//    of two, in the multiply-add that removes the INT8 offset). Both tiles use it.
+//  - warp 12: one thread issues the products, S of the next page before P V of
+//    this, tile by tile, so that one tile's softmax runs beside the other's
+//    products. (Issued by a conversion warp, the two waited for each other: 1.05 ms
+//    instead of the figure below.)
+// f32 rows take two halves for Q and for P (22 bits): twice the products.
 //
-// Bound by issue: per page and tile about 2600 warp instructions of softmax and
-// 1000 of conversion against 511 cycles of products.
-//
-// Waits are bounded (2 s of %globaltimer); on expiry the CTA raises an error word,
+// Waits are bounded (4e9 clocks, about 2 s); on expiry the CTA raises an error word,
 // stops, waits (bounded) for its own products, frees TMEM and exits.
 #include <math.h>
 
@@ -41,9 +41,10 @@ namespace {
 
 __device__ int g_kv8_error = 0;
 
-constexpr int kRows = kKv8Long;          // query rows of a tile
-constexpr int kThreads = 9 * 32;
-constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr int kRows = 128;               // query rows of a tile
+constexpr int kPair = kKv8Long;          // of a CTA's two tiles
+constexpr int kThreads = 13 * 32;
+constexpr long long kWaitClocks = 4000000000ll;   // about 2 s
 constexpr float kVUp = 32.0f;            // V enters as 2^5 code / largest scale: 1152 2^5, the offset, is a half
 
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -62,27 +63,22 @@ __device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t par) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ unsigned long long gtime() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __noinline__ bool mb_wait_slow(uint64_t* b, uint32_t par) {
-    const unsigned long long t0 = gtime();
+__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t par) {
+    if (mb_try(b, par)) return true;
+    const long long t0 = clock64();
     while (!mb_try(b, par))
-        if (gtime() - t0 > kWaitNs) {
+        if (clock64() - t0 > kWaitClocks) {
             atomicOr(&g_kv8_error, 1);
             return false;
         }
     return true;
 }
-__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t par) { return mb_try(b, par) || mb_wait_slow(b, par); }
-
-// By a whole warp: one lane waits.
+// By a whole warp: every lane polls, so that the warp stays together (one lane
+// polling for the others left it in two pieces that ran the code after it in turn:
+// 3 times the time per page).
 __device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t par) {
-    int ok = 1;
-    if ((threadIdx.x & 31) == 0) ok = mb_wait(b, par) ? 1 : 0;
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    const bool ok = mb_wait(b, par);
+    return __all_sync(0xffffffffu, ok);
 }
 
 // The largest V scale of a page's blocks that hold positions below end.
@@ -130,6 +126,16 @@ __device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, boo
         "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
+// The same with A in TMEM: a row is a lane, a column holds two consecutive values.
+template <int N>
+__device__ __forceinline__ void umma_f16_ta(uint32_t d, uint32_t a, uint64_t b, bool acc) {
+    constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
 __device__ __forceinline__ void umma_commit(uint64_t* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(b))
                  : "memory");
@@ -149,18 +155,35 @@ __device__ __forceinline__ void tmem_ld32(uint32_t ta, float* f) {
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(ta));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t ta, const float* f) {
+__device__ __forceinline__ void tmem_ld16(uint32_t ta, float* f) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(ta));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t ta, const float* f) {
     const uint32_t* v = reinterpret_cast<const uint32_t*>(f);
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(ta),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(ta),
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st8(uint32_t ta, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(ta), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+// After the wait the loaded values pass through an empty statement, so that no
+// use of them moves before it.
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(float (&f)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+f"(f[i]));
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -194,48 +217,59 @@ template <int HD, bool F32>
 struct Layout {
     static constexpr int kCb = (HD + 63) / 64;                 // 64-dimension column blocks
     static constexpr int kParts = F32 ? 2 : 1;                 // halves per value of Q and P
-    static constexpr int kQ = 0, kQPart = kCb * kRows * 128;
-    static constexpr int kK = kQ + kParts * kQPart;
-    static constexpr int kV = kK + kCb * kPageSize * 128;
-    static constexpr int kP = kV + HD * 128, kPPart = kRows * 128;
-    static constexpr int kBytes = kP + kParts * kPPart + 1024;
+    static constexpr int kQPart = kCb * kRows * 128, kQTile = kParts * kQPart;
+    static constexpr int kKStage = kCb * kPageSize * 128, kVStage = HD * 128;
+    static constexpr int kQ = 0, kK = 2 * kQTile, kV = kK + 2 * kKStage;
+    static constexpr int kBytes = kV + 2 * kVStage + 1024;
+};
+
+// What a tile's warps and the issuing thread signal to each other. p_full is by
+// buffer, as s_full: a warp may write the next page's P before a slower one has
+// written this page's, and the barrier must not count its arrival for that one.
+struct TileBars {
+    uint64_t q_full, s_full[2], p_full[2], pv_done;
 };
 
 template <int HD, int DT, bool E4M3>
-__global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 1)
     kv8_prefill_kernel(const Kv8AttnParams p, const Kv8Tiles tl, const int vec) {
     constexpr bool F32 = DT == FL_F32;
     typedef Layout<HD, F32> L;
     constexpr int NC = HD / 32;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t k_full, k_empty, v_full, pv_done, p_full, s_full[2], s_empty[2];
+    __shared__ __align__(8) TileBars bars[2];
+    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     __shared__ uint32_t tmem_s;
     __shared__ int bad_s, last_s;
     __shared__ Kv8Item it;
     const uint32_t smem = (saddr(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mb_init(&k_full, 4);
-        mb_init(&k_empty, 1);
-        mb_init(&v_full, 4);
-        mb_init(&pv_done, 1);
-        mb_init(&p_full, 4);
         for (int i = 0; i < 2; i++) {
-            mb_init(&s_full[i], 1);
-            mb_init(&s_empty[i], 4);
+            mb_init(&bars[i].q_full, 4);
+            mb_init(&bars[i].s_full[0], 1);
+            mb_init(&bars[i].s_full[1], 1);
+            mb_init(&bars[i].p_full[0], 4);
+            mb_init(&bars[i].p_full[1], 4);
+            mb_init(&bars[i].pv_done, 1);
+            mb_init(&k_full[i], 4);
+            mb_init(&k_empty[i], 1);
+            mb_init(&v_full[i], 4);
+            mb_init(&v_empty[i], 1);
         }
         bad_s = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(saddr(&tmem_s)));
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&tmem_s)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_s;
-    uint32_t J0 = 0;   // pages of the items before: the phases of the barriers run on
+    // pages and items before, of the CTA and of either tile: the barriers' phases run on
+    uint32_t J0 = 0, jt0 = 0, jt1 = 0, items0 = 0, items1 = 0;
 
     for (long long x = -1;;) {
         if (warp == 0) next_item(p, tl, x, lane, it);
@@ -243,19 +277,22 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
         if (it.pages == 0 || bad_s) break;
         x = it.next;
         const int h = it.head, ctx = it.ctx, row0 = it.row0, nb = it.nb;
-        const int np = min(kRows, nb * p.group - it.tile * kRows);
-        const int tok_last = (it.tile * kRows + np - 1) / p.group;
+        const int np = min(kPair, nb * p.group - it.tile * kPair);
+        const int nt = np > kRows ? 2 : 1;                   // tiles with rows
+        const int tok_last = (it.tile * kPair + np - 1) / p.group;
         const int kend = p.mask ? ctx + nb : ctx + tok_last + 1;
         const int k0 = it.page0 * kPageSize;                 // first key of the range
         const int n = max(0, min(it.pages, (kend - k0 + kPageSize - 1) / kPageSize));
         const int* bt = p.t.block_table + (size_t)it.seq * p.max_pages + it.page0;
 
-        if (warp < 4) {
+        if (warp < 4 * nt) {
             // ------------------------------------------------------- softmax
-            const int r = threadIdx.x;
-            const int pr = it.tile * kRows + r, tok = pr / p.group;
+            const int tile = warp >> 2, r = threadIdx.x & (kRows - 1);
+            TileBars& bar = bars[tile];
+            const uint32_t jb = tile ? jt1 : jt0;
+            const int pr = it.tile * kPair + threadIdx.x, tok = pr / p.group;
             const int head = h * p.group + pr - tok * p.group, row = row0 + tok;
-            const bool live = r < np && row < p.rows;
+            const bool live = threadIdx.x < np && row < p.rows;
             const size_t qat = (size_t)row * p.ldq + (size_t)head * HD;
             float amax = 0.0f;
             if (live) {
@@ -276,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
                 if (live) load8<DT>(p.q, qat + 8 * c, vec, f);
 #pragma unroll
                 for (int j = 0; j < 8; j++) f[j] *= qs;
-                const uint32_t a = smem + L::kQ + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                const uint32_t a = smem + L::kQ + tile * L::kQTile + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                 sts16(a, h2(f[0], f[1]), h2(f[2], f[3]), h2(f[4], f[5]), h2(f[6], f[7]));
                 if constexpr (F32) {
 #pragma unroll
@@ -287,62 +324,53 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
             proxy_fence();
             __syncwarp();
             bool ok = true;
-            // Q is there and both S buffers are free: s_empty grants pages J0 and J0 + 1
-            if (lane == 0 && n > 0) mb_arrive(&s_empty[J0 & 1]);
-            if (lane == 0 && n > 1) mb_arrive(&s_empty[(J0 + 1) & 1]);
-            const uint32_t tq = tmem + ((uint32_t)(32 * warp) << 16);
+            if (lane == 0 && n > 0) mb_arrive(&bar.q_full);
+            const uint32_t tq = tmem + tile * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
             float m = -INFINITY, l = 0.0f, vref = 0.0f;
             const int lim = p.mask ? ctx + nb : ctx + tok + 1;   // positions this row may see
-            const uint8_t* mrow = p.mask && live ? p.mask + (size_t)row * p.ldm : nullptr;
+            // dead rows read some row of the mask, to no effect
+            const uint8_t* mrow = p.mask + (size_t)(live ? row : min(row0, p.rows - 1)) * p.ldm;
             Scales next(p, bt, h, n);
             for (int j = 0; j < n; j++) {
-                const uint32_t J = J0 + j;
+                const uint32_t J = jb + j;
                 const float4 ks4 = next.k;
                 const float vs = vscale_max(next.v, k0 + j * kPageSize, ctx + nb);
                 next.load(p, bt, h, j + 1, n);
-                if (!warp_wait(&s_full[J & 1], (J >> 1) & 1)) { ok = false; break; }
+                if (!warp_wait(&bar.s_full[J & 1], (J >> 1) & 1)) { ok = false; break; }
                 tc_after();
-                // S twice, 32 columns at a time: 64 values would not stay in registers
                 const uint32_t sb = tq + (J & 1) * 64;
-                const float f[4] = {ks4.x * unshift, ks4.y * unshift, ks4.z * unshift, ks4.w * unshift};
+                float s[64];
+                tmem_ld32(sb, s);
+                tmem_ld32(sb + 32, s + 32);
+                float f[4] = {ks4.x * unshift, ks4.y * unshift, ks4.z * unshift, ks4.w * unshift};
                 const int kb = k0 + j * kPageSize;
-                const bool part = kb + kPageSize > ctx + (p.mask ? 0 : it.tile * kRows / p.group);
-                // bit i: this row sees column i
-                uint32_t see[2] = {0xffffffffu, 0xffffffffu};
-                if (part) {
-                    const int left = lim - kb;
-                    see[0] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-                    see[1] = left >= 64 ? 0xffffffffu : left <= 32 ? 0u : (1u << (left - 32)) - 1u;
-                    if (p.mask) {
-                        unsigned long long hide = 0;
-                        for (int i = max(0, ctx - kb); i < min(64, left); i++)
-                            if (!mrow || mrow[kb + i - ctx] == 0) hide |= 1ull << i;
-                        see[0] &= ~(uint32_t)hide;
-                        see[1] &= ~(uint32_t)(hide >> 32);
-                    }
-                }
+                const bool part = kb + kPageSize > ctx + (p.mask ? 0 : (it.tile * kPair + tile * kRows) / p.group);
+                tmem_wait_ld(s);
+                tc_before();
                 float mx = -INFINITY;
+                if (part) {
+                    const int left = lim - kb;   // columns of this page the row may see
+                    unsigned long long hide = 0;
+                    if (p.mask)
+                        for (int i = max(0, ctx - kb); i < min(64, left); i++)
+                            hide |= (unsigned long long)(mrow[kb + i - ctx] == 0) << i;
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    float s[32];
-                    tmem_ld32(sb + 32 * w, s);
-                    tmem_wait_ld();
-                    if (part) {
+                    for (int i = 0; i < 64; i++) {
+                        s[i] = i < left && !((hide >> i) & 1) ? s[i] * f[i >> 4] : -INFINITY;
+                        mx = fmaxf(mx, s[i]);
+                    }
 #pragma unroll
-                        for (int i = 0; i < 32; i++)
-                            mx = fmaxf(mx, (see[w] >> i) & 1 ? s[i] * f[2 * w + (i >> 4)] : -INFINITY);
-                    } else {
+                    for (int b = 0; b < 4; b++) f[b] = 1.0f;
+                } else {
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            float bm = s[16 * b];
+                    for (int b = 0; b < 4; b++) {
+                        float bm = s[16 * b];
 #pragma unroll
-                            for (int i = 1; i < 16; i++) bm = fmaxf(bm, s[16 * b + i]);
-                            mx = fmaxf(mx, bm * f[2 * w + b]);
-                        }
+                        for (int i = 1; i < 16; i++) bm = fmaxf(bm, s[16 * b + i]);
+                        mx = fmaxf(mx, bm * f[b]);
                     }
                 }
-                // P's buffer, and O: the products of the page before have to be done
-                if (j > 0 && !warp_wait(&pv_done, (J - 1) & 1)) { ok = false; break; }
+                __syncwarp();   // the TMEM accesses below take whole warps
                 const float vnew = fmaxf(vref, vs);
                 const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
                 if (j == 0) {
@@ -353,66 +381,61 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
                     m = mn;
                     l *= al;
                     const float g = al * (vref * pow2_inv(vnew));
+                    // O: the products of the page before have to be done
+                    if (!warp_wait(&bar.pv_done, (J - 1) & 1)) { ok = false; break; }
                     tc_after();
+#pragma unroll 1
+                    for (int c = 0; c < 2 * NC; c++) {
+                        float o[16];
+                        tmem_ld16(tq + 128 + 16 * c, o);
+                        tmem_wait_ld(o);
 #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        float o[32];
-                        tmem_ld32(tq + 128 + 32 * c, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] *= g;
-                        tmem_st32(tq + 128 + 32 * c, o);
+                        for (int i = 0; i < 16; i++) o[i] *= g;
+                        tmem_st16(tq + 128 + 16 * c, o);
                     }
                     tmem_wait_st();
                 }
                 vref = vnew;
                 const float mr = m == -INFINITY ? 0.0f : m - kShift;
-                const uint32_t pa = smem + L::kP + r * 128;
+                // P over S in TMEM, two halves a column (f32 rows: the remainders behind)
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    float s[32];
-                    tmem_ld32(sb + 32 * w, s);
-                    tmem_wait_ld();
+                for (int c = 0; c < 4; c++) {
+                    uint32_t hi[8], lo[F32 ? 8 : 1];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float e[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            e[i] = ex2(__fmaf_rn(s[8 * c + i], f[2 * w + (c >> 1)], -mr));
-                            if (part && !((see[w] >> (8 * c + i)) & 1)) e[i] = 0.0f;
-                            l += e[i];
-                        }
-                        const uint32_t a = pa + (((4 * w + c) ^ (r & 7)) << 4);
-                        sts16(a, h2(e[0], e[1]), h2(e[2], e[3]), h2(e[4], e[5]), h2(e[6], e[7]));
+                    for (int i = 0; i < 8; i++) {
+                        float e0 = ex2(__fmaf_rn(s[16 * c + 2 * i], f[c], -mr));
+                        float e1 = ex2(__fmaf_rn(s[16 * c + 2 * i + 1], f[c], -mr));
+                        l += e0 + e1;
+                        hi[i] = h2(e0, e1);
                         if constexpr (F32) {
-#pragma unroll
-                            for (int i = 0; i < 8; i++) e[i] -= __half2float(__float2half_rn(e[i]));
-                            sts16(a + L::kPPart, h2(e[0], e[1]), h2(e[2], e[3]), h2(e[4], e[5]), h2(e[6], e[7]));
+                            e0 -= __half2float(__float2half_rn(e0));
+                            e1 -= __half2float(__float2half_rn(e1));
+                            lo[i] = h2(e0, e1);
                         }
                     }
+                    tmem_st8(sb + 8 * c, hi);
+                    if constexpr (F32) tmem_st8(sb + 32 + 8 * c, lo);
                 }
+                tmem_wait_st();
                 tc_before();
                 __syncwarp();
-                if (lane == 0 && j + 2 < n) mb_arrive(&s_empty[J & 1]);   // S is read: free for page J + 2
-                proxy_fence();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mb_arrive(&p_full);
+                if (lane == 0) mb_arrive(&bar.p_full[J & 1]);
             }
             // the row's output: normalised, to its place or to the part's slot
-            if (ok && n > 0) ok = warp_wait(&pv_done, (J0 + n - 1) & 1);
+            if (ok && n > 0) ok = warp_wait(&bar.pv_done, (jb + n - 1) & 1);
             if (!ok) {
                 if (lane == 0) atomicOr(&bad_s, 1);
             } else {
                 tc_after();
                 const size_t slot = 2 * (size_t)blockIdx.x + (it.split == 0);
                 const float g = l != 0.0f ? __fdiv_rn(vref * (1.0f / kVUp), l) : 0.0f;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < NC; c++) {
                     float o[32];
+                    __syncwarp();   // rows without an output left the stores early
                     if (n > 0) {
                         tmem_ld32(tq + 128 + 32 * c, o);
-                        tmem_wait_ld();
+                        tmem_wait_ld(o);
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
@@ -420,18 +443,18 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
 #pragma unroll
                         for (int k = 0; k < 4; k++) v[k] = n > 0 && l != 0.0f ? o[i + k] * g : 0.0f;
                         if (it.splits > 1)
-                            *reinterpret_cast<float4*>(tl.part + (slot * kRows + r) * HD + c * 32 + i) =
+                            *reinterpret_cast<float4*>(tl.part + (slot * kPair + threadIdx.x) * HD + c * 32 + i) =
                                 make_float4(v[0], v[1], v[2], v[3]);
                         else if (live)
                             store4<DT>(p.out, (size_t)row * p.ldo + (size_t)head * HD + c * 32 + i, vec, v);
                     }
                 }
-                if (it.splits > 1) tl.part_ml[slot * kRows + r] = make_float2(m, l);
+                if (it.splits > 1) tl.part_ml[slot * kPair + threadIdx.x] = make_float2(m, l);
                 tc_before();
             }
-        } else if (warp < 8) {
+        } else if (warp >= 8 && warp < 12) {
             // ---------------------------------------------------- conversion
-            const int blk = warp - 4, t4 = lane & 3, g = lane >> 2;
+            const int blk = warp - 8, t4 = lane & 3, g = lane >> 2;
             // the next page's K codes are loaded once this page's are converted, and
             // its V codes likewise; page numbers and scales a page ahead
             uint4 kq[NC], vq[NC];
@@ -446,23 +469,8 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
 #pragma unroll
                 for (int c = 0; c < NC; c++) vq[c] = ld_stream16(p.v + off + c * 512);
             };
-            float vref = 0.0f;
-            bool ok = true;
-            if (n > 0) {
-                load_k(bt[0]);
-                load_v();
-            }
-            for (int j = 0; j < n; j++) {
-                const uint32_t J = J0 + j;
-                const float4 vs4 = next.v;
-                const int after = next.page;   // of page j + 1
-                next.load(p, bt, h, j + 1, n);
-                const int kb = k0 + j * kPageSize + blk * kKv8Block;
-                vref = fmaxf(vref, vscale_max(vs4, k0 + j * kPageSize, ctx + nb));
-                const float vs = blk < 2 ? (blk ? vs4.y : vs4.x) : (blk == 2 ? vs4.z : vs4.w);
-                const float ratio = kb < ctx + nb ? vs * pow2_inv(vref) * kVUp : 0.0f;
-                if (J > 0 && !warp_wait(&k_empty, (J - 1) & 1)) { ok = false; break; }
-                // K rows: key 16 blk + 4 (g / 2) + (g & 1) + 2 half, dimensions 32 c + 8 t4 .. + 7
+            // K rows: key 16 blk + 4 (g / 2) + (g & 1) + 2 half, dimensions 32 c + 8 t4 .. + 7
+            auto write_k = [&](uint32_t st) {
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     const uint32_t w[4] = {kq[c].x, kq[c].y, kq[c].z, kq[c].w};
@@ -472,81 +480,124 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
                         codes_to_halves<E4M3>(w[2 * half], a, b);
                         codes_to_halves<E4M3>(w[2 * half + 1], d, e);
                         const int key = blk * kKv8Block + 4 * (g >> 1) + (g & 1) + 2 * half;
-                        sts16(smem + L::kK + (c >> 1) * (kPageSize * 128) + key * 128 +
+                        sts16(smem + L::kK + st * L::kKStage + (c >> 1) * (kPageSize * 128) + key * 128 +
                                   (((((c & 1) << 2) + t4) ^ (key & 7)) << 4), a, b, d, e);
                     }
                 }
                 proxy_fence();
                 __syncwarp();
-                if (lane == 0) mb_arrive(&k_full);
-                if (j + 1 < n) load_k(after);
-                if (J > 0 && !warp_wait(&pv_done, (J - 1) & 1)) { ok = false; break; }
-                // V^T rows: dimension 32 c + 4 g + i, keys 16 blk + 4 t4 .. + 3; positions
-                // behind the sequence may hold anything, an E4M3 NaN too
+                if (lane == 0) mb_arrive(&k_full[st]);
+            };
+            // V^T rows: dimension 32 c + 4 g + i, keys 16 blk + 4 t4 .. + 3; positions
+            // behind the sequence may hold anything, an E4M3 NaN too
+            float vref = 0.0f;
+            auto write_v = [&](uint32_t st, int j, const float4& vs4) {
+                const int kb = k0 + j * kPageSize + blk * kKv8Block;
+                vref = fmaxf(vref, vscale_max(vs4, k0 + j * kPageSize, ctx + nb));
+                const float vs = blk < 2 ? (blk ? vs4.y : vs4.x) : (blk == 2 ? vs4.z : vs4.w);
+                const float ratio = kb < ctx + nb ? vs * pow2_inv(vref) * kVUp : 0.0f;
                 const int left = ctx + nb - kb - 4 * t4;
                 const uint32_t keep = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-                const __half2 rr = __floats2half2_rn(ratio, ratio), off = __floats2half2_rn(-1152.0f * ratio, -1152.0f * ratio);
+                const __half2 rr = __floats2half2_rn(ratio, ratio), ro = __floats2half2_rn(-1152.0f * ratio, -1152.0f * ratio);
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     const uint32_t w[4] = {vq[c].x, vq[c].y, vq[c].z, vq[c].w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         uint32_t a, b;
-                        scaled_halves<E4M3>(E4M3 ? w[i] & keep : w[i], rr, off, a, b);
+                        scaled_halves<E4M3>(E4M3 ? w[i] & keep : w[i], rr, ro, a, b);
                         const int d = c * 32 + 4 * g + i;
-                        sts8(smem + L::kV + d * 128 + (((2 * blk + (t4 >> 1)) ^ (d & 7)) << 4) + (t4 & 1) * 8, a, b);
+                        sts8(smem + L::kV + st * L::kVStage + d * 128 + (((2 * blk + (t4 >> 1)) ^ (d & 7)) << 4) + (t4 & 1) * 8, a, b);
                     }
                 }
                 proxy_fence();
                 __syncwarp();
-                if (lane == 0) mb_arrive(&v_full);
+                if (lane == 0) mb_arrive(&v_full[st]);
+            };
+            bool ok = true;
+            if (n > 0) {
+                load_k(bt[0]);
+                load_v();
+            }
+            for (int j = 0; j < n; j++) {
+                const uint32_t J = J0 + j, st = J & 1, par = ((J >> 1) - 1) & 1;
+                const float4 vs4 = next.v;
+                const int after = next.page;   // of page j + 1
+                next.load(p, bt, h, j + 1, n);
+                if (J > 1 && !warp_wait(&k_empty[st], par)) { ok = false; break; }
+                write_k(st);
+                if (j + 1 < n) load_k(after);
+                if (J > 1 && !warp_wait(&v_empty[st], par)) { ok = false; break; }
+                write_v(st, j, vs4);
                 if (j + 1 < n) load_v();
             }
             if (!ok && lane == 0) atomicOr(&bad_s, 1);
-        } else if (lane == 0) {
+        } else if (warp == 12 && lane == 0) {
             // ------------------------------------------------------ products
-            bool ok = true;
-            uint32_t nqk = J0, npv = J0;   // pages whose products are issued
-            auto scores = [&](uint32_t J) -> bool {   // S of page J into buffer J & 1
-                if (!mb_wait(&s_empty[J & 1], (J >> 1) & 1) || !mb_wait(&k_full, J & 1)) return false;
+            auto scores = [&](int tile, int j) -> bool {   // S of page j of a tile
+                const uint32_t J = J0 + j, T = (tile ? jt1 : jt0) + j;
+                // over P of the tile's page before last: its product has to be done (the
+                // items before are; their phase could be mistaken for a later one's)
+                if (j > 1 && !mb_wait(&bars[tile].pv_done, (T - 2) & 1)) return false;
+                if (j == 0 && !mb_wait(&bars[tile].q_full, (tile ? items1 : items0) & 1)) return false;
+                if (!mb_wait(&k_full[J & 1], (J >> 1) & 1)) return false;
                 tc_after();
 #pragma unroll
                 for (int q = 0; q < L::kParts; q++)
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++)
-                        umma_f16<kPageSize>(tmem + (J & 1) * 64,
-                                            desc_sw128(smem + L::kQ + q * L::kQPart + (k >> 2) * (kRows * 128) + (k & 3) * 32),
-                                            desc_sw128(smem + L::kK + (k >> 2) * (kPageSize * 128) + (k & 3) * 32),
+                        umma_f16<kPageSize>(tmem + tile * 256 + (T & 1) * 64,
+                                            desc_sw128(smem + L::kQ + tile * L::kQTile + q * L::kQPart +
+                                                       (k >> 2) * (kRows * 128) + (k & 3) * 32),
+                                            desc_sw128(smem + L::kK + (J & 1) * L::kKStage +
+                                                       (k >> 2) * (kPageSize * 128) + (k & 3) * 32),
                                             q + k > 0);
-                umma_commit(&k_empty);
-                umma_commit(&s_full[J & 1]);
-                nqk = J + 1;
+                umma_commit(&bars[tile].s_full[T & 1]);
+                if (tile == nt - 1) umma_commit(&k_empty[J & 1]);
                 return true;
             };
-            if (n > 0) ok = scores(J0);
-            for (int j = 0; j < n && ok; j++) {
-                const uint32_t J = J0 + j;
-                if (j + 1 < n && !scores(J + 1)) { ok = false; break; }
-                if (!mb_wait(&p_full, J & 1) || !mb_wait(&v_full, J & 1)) { ok = false; break; }
+            auto output = [&](int tile, int j) -> bool {   // O (+)= P V of page j of a tile
+                const uint32_t J = J0 + j, T = (tile ? jt1 : jt0) + j;
+                if (!mb_wait(&v_full[J & 1], (J >> 1) & 1) || !mb_wait(&bars[tile].p_full[T & 1], (T >> 1) & 1)) return false;
                 tc_after();
 #pragma unroll
                 for (int q = 0; q < L::kParts; q++)
 #pragma unroll
                     for (int k = 0; k < kPageSize / 16; k++)
-                        umma_f16<HD>(tmem + 128, desc_sw128(smem + L::kP + q * L::kPPart + k * 32),
-                                     desc_sw128(smem + L::kV + k * 32), j > 0 || q + k > 0);
-                umma_commit(&pv_done);
-                npv = J + 1;
+                        umma_f16_ta<HD>(tmem + tile * 256 + 128, tmem + tile * 256 + (T & 1) * 64 + q * 32 + k * 8,
+                                        desc_sw128(smem + L::kV + (J & 1) * L::kVStage + k * 32), j > 0 || q + k > 0);
+                umma_commit(&bars[tile].pv_done);
+                if (tile == nt - 1) umma_commit(&v_empty[J & 1]);
+                return true;
+            };
+            bool ok = true;
+            int nqk = 0, npv = 0;   // pages whose products are issued, of all tiles
+            if (n > 0)
+                ok = scores(0, 0) && (nt == 1 || scores(1, 0));
+            nqk = ok && n > 0;
+            for (int j = 0; j < n && ok; j++) {
+                ok = (j + 1 >= n || scores(0, j + 1)) && output(0, j);
+                if (nt > 1) ok = ok && (j + 1 >= n || scores(1, j + 1)) && output(1, j);
+                if (ok) {
+                    nqk = min(j + 2, n);
+                    npv = j + 1;
+                }
             }
             if (!ok) {   // the products under way read this CTA's memory: wait for them, too
-                if (nqk > J0) (void)mb_wait(&k_empty, (nqk - 1) & 1);
-                if (npv > J0) (void)mb_wait(&pv_done, (npv - 1) & 1);
+                if (nqk > 0) (void)mb_wait(&k_empty[(J0 + nqk - 1) & 1], ((J0 + nqk - 1) >> 1) & 1);
+                if (npv > 0) (void)mb_wait(&v_empty[(J0 + npv - 1) & 1], ((J0 + npv - 1) >> 1) & 1);
                 atomicOr(&bad_s, 1);
             }
         }
         __syncthreads();
         if (bad_s) break;
         J0 += n;
+        jt0 += n;
+        items0 += n > 0;
+        if (nt > 1) {
+            jt1 += n;
+            items1 += n > 0;
+        }
         if (it.splits > 1) {
             // the last range to arrive joins the tile's ranges, in their order
             int* cnt = tl.part_cnt + it.part;
@@ -559,8 +610,8 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
                 for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kThreads) {
                     const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
                     float acc[4];
-                    join_parts(tl, it, kRows, HD, r, d, acc);
-                    const int pr = it.tile * kRows + r, tk = pr / p.group;
+                    join_parts(tl, it, kPair, HD, r, d, acc);
+                    const int pr = it.tile * kPair + r, tk = pr / p.group;
                     const int hq = h * p.group + pr - tk * p.group;
                     if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
                 }
@@ -570,9 +621,9 @@ __global__ void __launch_bounds__(kThreads, DT == FL_F32 ? 1 : 2)
         __syncthreads();
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 12) {
         tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
 }
 
@@ -598,14 +649,10 @@ cudaError_t with_kernel(int hd, int type, int dtype, F f) {
 
 }  // namespace
 
-int kv8_prefill_occupancy(int head_dim, int type, int dtype) {
-    int n = 0;
-    with_kernel(head_dim, type, dtype, [&](auto* k, int smem) {
-        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, smem);
-        return e;
+cudaError_t kv8_prefill_prepare(int head_dim, int type, int dtype) {
+    return with_kernel(head_dim, type, dtype, [&](auto* k, int smem) {
+        return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
-    return std::min(std::max(n, 1), 2);   // TMEM: 256 of 512 columns each
 }
 
 cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s) {
