@@ -339,38 +339,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!warp_wait(&bar.s_full[J & 1], (J >> 1) & 1)) { ok = false; break; }
                 tc_after();
                 const uint32_t sb = tq + (J & 1) * 64;
-                float s[64];
-                tmem_ld32(sb, s);
-                tmem_ld32(sb + 32, s + 32);
-                float f[4] = {ks4.x * unshift, ks4.y * unshift, ks4.z * unshift, ks4.w * unshift};
+                const float f[4] = {ks4.x * unshift, ks4.y * unshift, ks4.z * unshift, ks4.w * unshift};
                 const int kb = k0 + j * kPageSize;
                 const bool part = kb + kPageSize > ctx + (p.mask ? 0 : (it.tile * kPair + tile * kRows) / p.group);
-                tmem_wait_ld(s);
-                tc_before();
-                float mx = -INFINITY;
+                uint32_t see0 = 0xffffffffu, see1 = 0xffffffffu;   // columns of this page the row sees
                 if (part) {
-                    const int left = lim - kb;   // columns of this page the row may see
-                    unsigned long long hide = 0;
+                    const int left = lim - kb;
+                    unsigned long long b = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1ull;
                     if (p.mask)
                         for (int i = max(0, ctx - kb); i < min(64, left); i++)
-                            hide |= (unsigned long long)(mrow[kb + i - ctx] == 0) << i;
-#pragma unroll
-                    for (int i = 0; i < 64; i++) {
-                        s[i] = i < left && !((hide >> i) & 1) ? s[i] * f[i >> 4] : -INFINITY;
-                        mx = fmaxf(mx, s[i]);
-                    }
-#pragma unroll
-                    for (int b = 0; b < 4; b++) f[b] = 1.0f;
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        float bm = s[16 * b];
-#pragma unroll
-                        for (int i = 1; i < 16; i++) bm = fmaxf(bm, s[16 * b + i]);
-                        mx = fmaxf(mx, bm * f[b]);
-                    }
+                            b &= ~((unsigned long long)(mrow[kb + i - ctx] == 0) << i);
+                    see0 = (uint32_t)b;
+                    see1 = (uint32_t)(b >> 32);
                 }
                 __syncwarp();   // the TMEM accesses below take whole warps
+                // S is read twice, 32 columns at a time: all 64 do not stay in registers
+                float mx = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    float s[32];
+                    tmem_ld32(sb + 32 * w, s);
+                    tmem_wait_ld(s);
+                    if (part) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++)
+                            mx = fmaxf(mx, ((w ? see1 : see0) >> i) & 1 ? s[i] * f[2 * w + (i >> 4)] : -INFINITY);
+                    } else {
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {
+                            float m0 = s[16 * b], m1 = s[16 * b + 1];
+#pragma unroll
+                            for (int i = 2; i < 16; i += 2) {
+                                m0 = fmaxf(m0, s[16 * b + i]);
+                                m1 = fmaxf(m1, s[16 * b + i + 1]);
+                            }
+                            mx = fmaxf(mx, fmaxf(m0, m1) * f[2 * w + b]);
+                        }
+                    }
+                }
                 const float vnew = fmaxf(vref, vs);
                 const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
                 if (j == 0) {
@@ -397,24 +403,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 vref = vnew;
                 const float mr = m == -INFINITY ? 0.0f : m - kShift;
-                // P over S in TMEM, two halves a column (f32 rows: the remainders behind)
+                // P over S in TMEM, two halves a column: 16 keys at columns 0, 8, 32 and 40
+                // (f32 rows: their remainders 16 columns further)
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t hi[8], lo[F32 ? 8 : 1];
+                for (int w = 0; w < 2; w++) {
+                    float s[32];
+                    tmem_ld32(sb + 32 * w, s);
+                    tmem_wait_ld(s);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        float e0 = ex2(__fmaf_rn(s[16 * c + 2 * i], f[c], -mr));
-                        float e1 = ex2(__fmaf_rn(s[16 * c + 2 * i + 1], f[c], -mr));
-                        l += e0 + e1;
-                        hi[i] = h2(e0, e1);
-                        if constexpr (F32) {
-                            e0 -= __half2float(__float2half_rn(e0));
-                            e1 -= __half2float(__float2half_rn(e1));
-                            lo[i] = h2(e0, e1);
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t hi[8], lo[F32 ? 8 : 1];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            float e0 = ex2(__fmaf_rn(s[16 * c + 2 * i], f[2 * w + c], -mr));
+                            float e1 = ex2(__fmaf_rn(s[16 * c + 2 * i + 1], f[2 * w + c], -mr));
+                            if (part) {
+                                e0 = ((w ? see1 : see0) >> (16 * c + 2 * i)) & 1 ? e0 : 0.0f;
+                                e1 = ((w ? see1 : see0) >> (16 * c + 2 * i + 1)) & 1 ? e1 : 0.0f;
+                            }
+                            l += e0 + e1;
+                            hi[i] = h2(e0, e1);
+                            if constexpr (F32) {
+                                e0 -= __half2float(__float2half_rn(e0));
+                                e1 -= __half2float(__float2half_rn(e1));
+                                lo[i] = h2(e0, e1);
+                            }
                         }
+                        tmem_st8(sb + 32 * w + 8 * c, hi);
+                        if constexpr (F32) tmem_st8(sb + 32 * w + 16 + 8 * c, lo);
                     }
-                    tmem_st8(sb + 8 * c, hi);
-                    if constexpr (F32) tmem_st8(sb + 32 + 8 * c, lo);
                 }
                 tmem_wait_st();
                 tc_before();
@@ -564,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int q = 0; q < L::kParts; q++)
 #pragma unroll
                     for (int k = 0; k < kPageSize / 16; k++)
-                        umma_f16_ta<HD>(tmem + tile * 256 + 128, tmem + tile * 256 + (T & 1) * 64 + q * 32 + k * 8,
+                        umma_f16_ta<HD>(tmem + tile * 256 + 128, tmem + tile * 256 + (T & 1) * 64 + q * 16 + (k >> 1) * 32 + (k & 1) * 8,
                                         desc_sw128(smem + L::kV + (J & 1) * L::kVStage + k * 32), j > 0 || q + k > 0);
                 umma_commit(&bars[tile].pv_done);
                 if (tile == nt - 1) umma_commit(&v_empty[J & 1]);
