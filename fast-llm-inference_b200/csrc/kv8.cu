@@ -16,18 +16,21 @@ namespace fl {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Plan: one kernel of one thread-block cluster. CTA 0 checks the lengths and
-// scans them; after a cluster barrier all CTAs return and take pages and write
-// the rows' maps and the work lists. Bound by latency: a chain of the length
-// loads, the scans and the page loads, with barriers between; the row maps of
-// a prompt batch are what the other CTAs are there for.
+// Plan: one kernel, of one CTA, or of one cluster of eight where a prompt batch
+// has rows for them. CTA 0 checks the lengths and scans them (each thread holds
+// one sequence while there are no more of them than threads); then all threads
+// return and take pages and write the row maps, item by item: an item's sequence
+// is found by bisection in the starts, which lie in shared memory up to
+// 1024 sequences. Bound by latency: the loads of the lengths, two barriers of the scan, the
+// page loads and stores with a barrier after each.
 // ---------------------------------------------------------------------------
-constexpr int kPT = 1024;
+constexpr int kSmSeqs = 1024;   // sequences whose starts shared memory holds
 
 // Packed query rows of a sequence (new rows x heads per kv head) from which the
-// prefill kernel takes it.
+// prefill kernel takes it: at 132 rows and 3700 keys (4 x 10 heads) it took 110 us,
+// the row kernel 84; at 3200 to 8200 rows 0.83 ms, the row kernel 2.47.
 #ifndef FL_KV8_LONG_MIN
-#define FL_KV8_LONG_MIN 40
+#define FL_KV8_LONG_MIN 192
 #endif
 constexpr int kLongMin = FL_KV8_LONG_MIN;
 
@@ -42,72 +45,6 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Exclusive prefix sum of one value per thread; the total to every thread.
-__device__ int block_scan(int v, int* red, int* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-    }
-    __syncthreads();
-    if (lane == 31) red[warp] = inc;
-    __syncthreads();
-    int w = red[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += y;
-    }
-    *total = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-    return (warp ? before : 0) + inc - v;
-}
-
-// The same of 64-bit numbers.
-__device__ long long block_scan64(long long v, long long* red, long long* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-    }
-    __syncthreads();
-    if (lane == 31) red[warp] = inc;
-    __syncthreads();
-    long long w = red[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += y;
-    }
-    *total = __shfl_sync(0xffffffffu, w, 31);
-    const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-    return (warp ? before : 0) + inc - v;
-}
-
-__device__ int block_max(int v, int* red) {
-    v = __reduce_max_sync(0xffffffffu, v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return __reduce_max_sync(0xffffffffu, red[threadIdx.x & 31]);
-}
-
-__device__ long long block_sum64(long long v, long long* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    long long t = red[threadIdx.x & 31];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    return t;
-}
-
 struct SeqPlan {
     int n, ctx, keep, need;   // new rows, cached positions, pages kept, pages held afterwards
     int rel;                  // pages returned
@@ -116,7 +53,7 @@ struct SeqPlan {
 
 __device__ __forceinline__ SeqPlan seq_plan(const PlanArgs& a, int b) {
     SeqPlan s;
-    const int nw = a.nw[b], held = __ldcg(a.t.held + b);
+    const int nw = a.nw[b], held = __ldcg(a.t.held + b), c = a.ctx[b];
     s.bad = false;
     s.n = max(nw, 0);
     s.ctx = 0;
@@ -124,7 +61,6 @@ __device__ __forceinline__ SeqPlan seq_plan(const PlanArgs& a, int b) {
     s.keep = nw < 0 ? 0 : held;
     s.need = s.keep;
     if (s.n > 0) {
-        const int c = a.ctx[b];
         const long long n = (long long)c + s.n;
         s.bad = c < 0 || s.n > a.max_new || n > (long long)a.max_pages * kPageSize;
         if (!s.bad) {
@@ -136,150 +72,199 @@ __device__ __forceinline__ SeqPlan seq_plan(const PlanArgs& a, int b) {
 }
 
 // The first index b with start[b + 1] > r, start ascending, start[nseq] > r.
-__device__ __forceinline__ int find_seq(const int* start, int nseq, int r) {
+template <class At>
+__device__ __forceinline__ int find_seq_by(int nseq, int r, At start) {
     int lo = 0, hi = nseq - 1;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (__ldcg(start + mid + 1) > r) hi = mid; else lo = mid + 1;
+        if (start(mid + 1) > r) hi = mid; else lo = mid + 1;
     }
     return lo;
 }
+// What is summed over the sequences, in the order of the scan.
+enum { V_ROWS, V_KEYS, V_REL, V_TAKE, V_UNITS, V_GBLK, V_TILES0, V_WORK0, V_TILES1, V_WORK1, V_COUNT };
 
-__global__ void __launch_bounds__(kPT) kv8_plan_kernel(const PlanArgs a) {
-    __shared__ int red[32];
-    __shared__ long long red64[32];
+__device__ __forceinline__ void add_seq(const PlanArgs& a, const SeqPlan& s, long long (&v)[V_COUNT], int (&mp)[2]) {
+    const int n = s.n ? s.ctx + s.n : 0;
+    v[V_ROWS] += s.n;
+    v[V_KEYS] += n;
+    v[V_REL] += s.rel;
+    v[V_TAKE] += s.need - s.keep;
+    v[V_UNITS] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
+    v[V_GBLK] += (n + kKv8Block - 1) / kKv8Block;
+    const int li = s.n * a.group >= a.long_min, tr = li ? kKv8Long : a.tile_rows;
+    const int tl = (s.n * a.group + tr - 1) / tr, pages = (n + kPageSize - 1) / kPageSize;
+    v[li ? V_TILES1 : V_TILES0] += tl;
+    v[li ? V_WORK1 : V_WORK0] += (long long)tl * pages;
+    mp[li] = max(mp[li], pages);
+}
+
+// starts of sequence b's shares
+__device__ __forceinline__ void put_starts(const Kv8Tables& t, int b, const long long (&v)[V_COUNT]) {
+    t.row_start[b] = (int)v[V_ROWS];
+    t.kv_start[b] = (int)v[V_KEYS];
+    t.rel_start[b] = (int)v[V_REL];
+    t.take_start[b] = (int)v[V_TAKE];
+    t.unit_start[b] = (int)v[V_UNITS];
+    t.gblk_start[b] = (int)v[V_GBLK];
+    t.tile_start[0][b] = v[V_TILES0];
+    t.work_start[0][b] = v[V_WORK0];
+    t.tile_start[1][b] = v[V_TILES1];
+    t.work_start[1][b] = v[V_WORK1];
+}
+
+template <int NT>
+__global__ void __launch_bounds__(NT) kv8_plan_kernel(const PlanArgs a) {
+    constexpr int NW = NT / 32;
+    __shared__ long long part[V_COUNT][NW];
+    __shared__ int part_mp[2][NW], bad_s[NW];
+    // row, release, take and unit starts, cached positions, pages kept
+    __shared__ int sm[6][kSmSeqs + 1];
     uint32_t rank, nrank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
     const Kv8Tables& t = a.t;
-    const int C = (a.nseq + kPT - 1) / kPT;
-    const int b0 = min(a.nseq, (int)threadIdx.x * C), b1 = min(a.nseq, b0 + C);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool local = a.nseq <= kSmSeqs;
     if (rank == 0) {
-        long long rows = 0, take = 0, rel = 0, bad = 0;
+        const int C = (a.nseq + NT - 1) / NT;
+        const int b0 = min(a.nseq, (int)threadIdx.x * C), b1 = min(a.nseq, b0 + C);
+        const int nfree = __ldcg(t.n_free);
+        SeqPlan one = {};
+        if (C == 1 && b0 < b1) one = seq_plan(a, b0);
+        auto plan = [&](int b) { return C == 1 ? one : seq_plan(a, b); };
+        long long own[V_COUNT] = {}, v[V_COUNT], tot[V_COUNT];
+        int mp[2] = {}, bad = 0;
         for (int b = b0; b < b1; b++) {
-            const SeqPlan s = seq_plan(a, b);
-            bad += s.bad;
-            rows += s.n;
-            take += s.need - s.keep;
-            rel += s.rel;
+            const SeqPlan s = plan(b);
+            bad |= s.bad;
+            add_seq(a, s, own, mp);
         }
-        bad = block_sum64(bad, red64);
-        rows = block_sum64(rows, red64);
-        take = block_sum64(take, red64);
-        rel = block_sum64(rel, red64);
-        const long long have = (long long)__ldcg(t.n_free) + rel;
-        const int st = bad > 0 || rows > a.max_rows ? -1 : take > have ? (int)min(take - have, 0x7fffffffll) : 0;
-        if (threadIdx.x == 0) *t.status = st;
+        // exclusive prefixes over the threads: within the warp, then over the warps
+#pragma unroll
+        for (int i = 0; i < V_COUNT; i++) {
+            long long inc = own[i];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            v[i] = inc - own[i];
+            if (lane == 31) part[i][warp] = inc;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int m = __reduce_max_sync(0xffffffffu, mp[i]);
+            if (lane == 0) part_mp[i][warp] = m;
+        }
+        bad = __any_sync(0xffffffffu, bad);
+        if (lane == 0) bad_s[warp] = bad;
+        __syncthreads();
+        bad = 0;
+        mp[0] = mp[1] = 0;
+#pragma unroll
+        for (int i = 0; i < V_COUNT; i++) tot[i] = 0;
+        for (int w = 0; w < NW; w++) {
+            bad |= bad_s[w];
+            mp[0] = max(mp[0], part_mp[0][w]);
+            mp[1] = max(mp[1], part_mp[1][w]);
+#pragma unroll
+            for (int i = 0; i < V_COUNT; i++) {
+                if (w == warp) v[i] += tot[i];
+                tot[i] += part[i][w];
+            }
+        }
+        const long long have = nfree + tot[V_REL];
+        const int st = bad || tot[V_ROWS] > a.max_rows ? -1
+                       : tot[V_TAKE] > have            ? (int)min(tot[V_TAKE] - have, 0x7fffffffll)
+                                                       : 0;
+        if (threadIdx.x == 0) {
+            *t.status = st;
+            *t.meta = st ? Kv8Meta{a.nseq, 0, 0, 0, 1, 0, {}}
+                         : Kv8Meta{a.nseq, (int)tot[V_ROWS], (int)tot[V_UNITS], (int)tot[V_GBLK], 0, 0,
+                                   {{tot[V_TILES0], tot[V_WORK0], mp[0]}, {tot[V_TILES1], tot[V_WORK1], mp[1]}}};
+        }
         if (st != 0) {
-            for (int b = threadIdx.x; b <= a.nseq; b += kPT) t.row_start[b] = t.kv_start[b] = 0;
-            if (threadIdx.x == 0) *t.meta = Kv8Meta{a.nseq, 0, 0, 0, 1, 0, {}};
+            for (int b = threadIdx.x; b <= a.nseq; b += NT) t.row_start[b] = t.kv_start[b] = 0;
         } else {
-            // sums of this thread's sequences, then the prefixes
-            int v[6] = {};
-            long long w[2] = {}, nt[2] = {};   // the attention's lists
-            int mp[2] = {};
             for (int b = b0; b < b1; b++) {
-                const SeqPlan s = seq_plan(a, b);
-                const int n = s.n ? s.ctx + s.n : 0;
-                v[0] += s.n;
-                v[1] += n;
-                v[2] += s.rel;
-                v[3] += s.need - s.keep;
-                v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
-                v[5] += (n + kKv8Block - 1) / kKv8Block;
-                const int li = s.n * a.group >= a.long_min, tr = li ? kKv8Long : a.tile_rows;
-                const int tl = (s.n * a.group + tr - 1) / tr, pages = (n + kPageSize - 1) / kPageSize;
-                nt[li] += tl;
-                w[li] += (long long)tl * pages;
-                mp[li] = max(mp[li], pages);
-            }
-            int tot[6];
-#pragma unroll
-            for (int i = 0; i < 6; i++) v[i] = block_scan(v[i], red, &tot[i]);
-            long long totw[2], tott[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                w[i] = block_scan64(w[i], red64, &totw[i]);
-                nt[i] = block_scan64(nt[i], red64, &tott[i]);
-                mp[i] = block_max(mp[i], red);
-            }
-            for (int b = b0; b < b1; b++) {
-                const SeqPlan s = seq_plan(a, b);
-                const int n = s.n ? s.ctx + s.n : 0;
+                const SeqPlan s = plan(b);
+                put_starts(t, b, v);
                 t.ctx[b] = s.ctx;
-                t.row_start[b] = v[0];
-                t.kv_start[b] = v[1];
-                t.rel_start[b] = v[2];
-                t.take_start[b] = v[3];
-                t.unit_start[b] = v[4];
-                t.gblk_start[b] = v[5];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    t.tile_start[i][b] = nt[i];
-                    t.work_start[i][b] = w[i];
+                if (local) {
+                    sm[0][b] = (int)v[V_ROWS];
+                    sm[1][b] = (int)v[V_REL];
+                    sm[2][b] = (int)v[V_TAKE];
+                    sm[3][b] = (int)v[V_UNITS];
+                    sm[4][b] = s.ctx;
+                    sm[5][b] = s.keep;
                 }
-                v[0] += s.n;
-                v[1] += n;
-                v[2] += s.rel;
-                v[3] += s.need - s.keep;
-                v[4] += s.n ? (n - 1) / kKv8Block - s.ctx / kKv8Block + 1 : 0;
-                v[5] += (n + kKv8Block - 1) / kKv8Block;
-                const int li = s.n * a.group >= a.long_min, tr = li ? kKv8Long : a.tile_rows;
-                const int tl = (s.n * a.group + tr - 1) / tr;
-                nt[li] += tl;
-                w[li] += (long long)tl * ((n + kPageSize - 1) / kPageSize);
+                add_seq(a, s, v, mp);
             }
             if (threadIdx.x == 0) {
-                t.row_start[a.nseq] = tot[0];
-                t.kv_start[a.nseq] = tot[1];
-                t.rel_start[a.nseq] = tot[2];
-                t.take_start[a.nseq] = tot[3];
-                t.unit_start[a.nseq] = tot[4];
-                t.gblk_start[a.nseq] = tot[5];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    t.tile_start[i][a.nseq] = tott[i];
-                    t.work_start[i][a.nseq] = totw[i];
+                put_starts(t, a.nseq, tot);
+                if (local) {
+                    sm[0][a.nseq] = (int)tot[V_ROWS];
+                    sm[1][a.nseq] = (int)tot[V_REL];
+                    sm[2][a.nseq] = (int)tot[V_TAKE];
+                    sm[3][a.nseq] = (int)tot[V_UNITS];
                 }
-                *t.meta = Kv8Meta{a.nseq, tot[0], tot[4], tot[5], 0, 0,
-                                  {{tott[0], totw[0], mp[0]}, {tott[1], totw[1], mp[1]}}};
             }
         }
     }
-    cluster_sync();
+    auto sync = [&]() {
+        if (nrank > 1) cluster_sync(); else __syncthreads();
+    };
+    sync();
     if (__ldcg(&t.meta->refused)) return;   // nothing changes (every CTA alike)
-    const int nfree = __ldcg(t.n_free), top = nfree + __ldcg(t.rel_start + a.nseq);
-    const int lane = threadIdx.x & 31;
-    const int wid = (int)rank * (kPT / 32) + (threadIdx.x >> 5), nw = (int)nrank * (kPT / 32);
-    // returned pages: the first page of the first sequence ends on top
-    for (int b = wid; b < a.nseq; b += nw)
-        if (a.nw[b] < 0) {
-            const int held = __ldcg(t.held + b), r0 = __ldcg(t.rel_start + b);
-            for (int j = lane; j < held; j += 32)
-                t.free_pages[top - 1 - r0 - j] = __ldcg(t.block_table + (size_t)b * a.max_pages + j);
+    if (local && rank > 0) {   // the other CTAs' copies
+        for (int b = threadIdx.x; b <= a.nseq; b += NT) {
+            sm[0][b] = __ldcg(t.row_start + b);
+            sm[1][b] = __ldcg(t.rel_start + b);
+            sm[2][b] = __ldcg(t.take_start + b);
+            sm[3][b] = __ldcg(t.unit_start + b);
+            if (b < a.nseq) {
+                sm[4][b] = __ldcg(t.ctx + b);
+                sm[5][b] = a.nw[b] < 0 ? 0 : __ldcg(t.held + b);
+            }
         }
-    cluster_sync();
-    // taken pages, and each sequence's shares of the work lists
-    for (int b = wid; b < a.nseq; b += nw) {
-        const SeqPlan s = seq_plan(a, b);
-        const int t0 = __ldcg(t.take_start + b);
-        for (int j = s.keep + lane; j < s.need; j += 32)
-            t.block_table[(size_t)b * a.max_pages + j] = __ldcg(t.free_pages + top - 1 - t0 - (j - s.keep));
-        __syncwarp();
-        if (lane == 0) t.held[b] = s.need;
-        if (!s.n) continue;
-        const int n = s.ctx + s.n;
-        const int r0 = __ldcg(t.row_start + b), u0 = __ldcg(t.unit_start + b);
-        const int units = (n - 1) / kKv8Block - s.ctx / kKv8Block + 1;
-        for (int u = lane; u < units; u += 32)
-            t.unit_row[u0 + u] = r0 + (u ? u * kKv8Block - s.ctx % kKv8Block : 0);
+        __syncthreads();
     }
-    cluster_sync();
-    if (rank == 0 && threadIdx.x == 0) *t.n_free = top - __ldcg(t.take_start + a.nseq);
-    const int rows = __ldcg(t.row_start + a.nseq);
-    for (int r = (int)rank * kPT + threadIdx.x; r < rows; r += (int)nrank * kPT) {
-        const int b = find_seq(t.row_start, a.nseq, r);
-        const int p = __ldcg(t.ctx + b) + r - __ldcg(t.row_start + b);
+    auto get = [&](int which, const int* g, int b) { return local ? sm[which][b] : __ldcg(g + b); };
+    auto keep_of = [&](int b) { return local ? sm[5][b] : a.nw[b] < 0 ? 0 : __ldcg(t.held + b); };
+    auto rows_at = [&](int b) { return get(0, t.row_start, b); };
+    auto rel_at = [&](int b) { return get(1, t.rel_start, b); };
+    auto take_at = [&](int b) { return get(2, t.take_start, b); };
+    auto unit_at = [&](int b) { return get(3, t.unit_start, b); };
+    const int i0 = (int)rank * NT + threadIdx.x, step = (int)nrank * NT;
+    const int nrel = rel_at(a.nseq), ntake = take_at(a.nseq), top = __ldcg(t.n_free) + nrel;
+    // returned pages: the first page of the first sequence ends on top
+    if (nrel) {
+        for (int i = i0; i < nrel; i += step) {
+            const int b = find_seq_by(a.nseq, i, rel_at);
+            t.free_pages[top - 1 - i] = __ldcg(t.block_table + (size_t)b * a.max_pages + i - rel_at(b));
+        }
+        sync();
+    }
+    for (int i = i0; i < ntake; i += step) {
+        const int b = find_seq_by(a.nseq, i, take_at);
+        t.block_table[(size_t)b * a.max_pages + keep_of(b) + i - take_at(b)] = __ldcg(t.free_pages + top - 1 - i);
+    }
+    const int nunit = unit_at(a.nseq);
+    for (int i = i0; i < nunit; i += step) {
+        const int b = find_seq_by(a.nseq, i, unit_at), u = i - unit_at(b);
+        t.unit_row[i] = rows_at(b) + (u ? u * kKv8Block - get(4, t.ctx, b) % kKv8Block : 0);
+    }
+    sync();
+    for (int b = i0; b < a.nseq; b += step) {   // a sequence without new rows has neither cached nor new pages to take
+        const int k = keep_of(b) + take_at(b + 1) - take_at(b);
+        t.held[b] = k;
+    }
+    if (i0 == 0) *t.n_free = top - ntake;
+    const int rows = rows_at(a.nseq);
+    for (int r = i0; r < rows; r += step) {
+        const int b = find_seq_by(a.nseq, r, rows_at);
+        const int p = get(4, t.ctx, b) + r - rows_at(b);
         t.pos[r] = p;
         t.row_seq[r] = b;
         t.slot[r] = __ldcg(t.block_table + (size_t)b * a.max_pages + p / kPageSize) * kPageSize + p % kPageSize;
@@ -471,7 +456,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_gather_kernel(const Gat
     for (long long w = (long long)blockIdx.x * kAppendWarps + (threadIdx.x >> 5); w < total;
          w += (long long)gridDim.x * kAppendWarps) {
         const int h = (int)((w >> 1) % a.kv_heads), g = (int)((w >> 1) / a.kv_heads);
-        const int b = find_seq(t.gblk_start, nseq, g);
+        // cached loads: the starts are an earlier kernel's (past L1 the search took most of the time)
+        const int b = find_seq_by(nseq, g, [&](int k) { return t.gblk_start[k]; });
         const int blk = g - t.gblk_start[b];
         const int k0 = t.kv_start[b] + blk * kKv8Block;
         const int m = min(kKv8Block, min(t.kv_start[b + 1], a.keys) - k0);
@@ -705,17 +691,18 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     a.long_min = kLongMin;
     // one CTA while its threads hold the rows; eight (a portable cluster) beyond
     const long long rows = std::min<long long>((long long)nseq * a.max_new, h->c.max_rows);
+    const bool small = nseq <= 256 && rows <= 1024;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = rows > 4 * kPT ? 8 : 1;
+    at[0].val.clusterDim.x = rows > 4096 ? 8 : 1;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(at[0].val.clusterDim.x);
-    cfg.blockDim = dim3(kPT);
+    cfg.blockDim = dim3(small ? 256 : 1024);
     cfg.stream = s;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
-    FL_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kv8_plan_kernel, a));
+    cfg.numAttrs = rows > 4096 ? 1 : 0;
+    FL_CHECK_CUDA(cudaLaunchKernelEx(&cfg, small ? kv8_plan_kernel<256> : kv8_plan_kernel<1024>, a));
     h->nseq = nseq;
     h->max_new = a.max_new;
     return FL_OK;
