@@ -95,23 +95,37 @@ __device__ __forceinline__ float pow2_inv(float s) {
     return __uint_as_float((254u << 23) - __float_as_uint(s));
 }
 
-// One code of y = x / scale, rounded to nearest even, beyond the largest code
-// to it (infinities too), NaN to zero. INT8 codes are stored plus 128.
+// Four codes of y = x / scale in a word, rounded to nearest even, beyond the
+// largest code to it (infinities too), NaN to zero. INT8 codes are stored plus
+// 128: y + 1.5 2^23 + 128 is y rounded, plus 128, in the low byte.
 template <bool E4M3>
-__device__ __forceinline__ uint8_t encode8(float y) {
-    if (y != y) y = 0.0f;
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    float y[4] = {a, b, c, d};
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = y[i] != y[i] ? 0.0f : y[i];
     if constexpr (E4M3) {
-        return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+        return lo | hi << 16;
     } else {
-        return (uint8_t)(__float2int_rn(fminf(fmaxf(y, -127.0f), 127.0f)) + 128);
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(y[i], -127.0f), 127.0f), 12583040.0f));
+        return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
     }
 }
+// The four values of a word's codes.
 template <bool E4M3>
-__device__ __forceinline__ float decode8(uint8_t c) {
+__device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {
     if constexpr (E4M3) {
-        return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+        const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)));
+        const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
+        f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
     } else {
-        return (float)((int)c - 128);
+        // byte u under 0x4b0000: the float 2^23 + u
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            f[i] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)), 8388736.0f);
     }
 }
 

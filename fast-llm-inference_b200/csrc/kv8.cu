@@ -313,15 +313,20 @@ template <bool V>
 __device__ __forceinline__ int piece_dim(int lane, int i) {
     return V ? (lane >> 2) * 4 : (lane & 3) * 8 + (i & 1) * 4;
 }
+// The bytes of word k that hold positions [first, first + m) of a block.
 template <bool V>
-__device__ __forceinline__ uint8_t piece_get(const uint32_t (&w)[4], int i, int j) {
-    return (uint8_t)(V ? w[j] >> (8 * i) : w[i] >> (8 * j));
-}
-template <bool V>
-__device__ __forceinline__ void piece_set(uint32_t (&w)[4], int i, int j, uint8_t c) {
-    uint32_t& x = V ? w[j] : w[i];
-    const int sh = 8 * (V ? i : j);
-    x = (x & ~(0xffu << sh)) | ((uint32_t)c << sh);
+__device__ __forceinline__ uint32_t piece_mask(int lane, int k, int first, int m) {
+    if (!V) {
+        const int p = piece_pos<false>(lane, k) - first;
+        return p >= 0 && p < m ? 0xffffffffu : 0u;
+    }
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int p = piece_pos<true>(lane, i) - first;
+        b |= p >= 0 && p < m ? 0xffu << (8 * i) : 0u;
+    }
+    return b;
 }
 
 // Rows x[0 .. m) (row stride ld) into positions first .. first + m of a block.
@@ -351,33 +356,42 @@ __device__ __forceinline__ void append_block(const void* x, size_t at, size_t ld
     const bool grew = s > s_old;
     const float inv = pow2_inv(s), ratio = __fmul_rn(s_old, inv);
     // a piece is written when it holds a new position, or an earlier one whose scale grew
-    bool fresh = false, old = false, gap = false;
+    uint32_t fresh[4], old[4];   // V: the same in every word
+    bool any_fresh = false, any_old = false, whole = true;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int p = piece_pos<V>(lane, i) - first;
-        fresh |= p >= 0 && p < m;
-        old |= p < 0;
-        gap |= p < 0 || p >= m;
+    for (int k = 0; k < 4; k++) {
+        fresh[k] = piece_mask<V>(lane, V ? 0 : k, first, m);
+        old[k] = piece_mask<V>(lane, V ? 0 : k, 0, first);
+        any_fresh |= fresh[k] != 0;
+        any_old |= old[k] != 0;
+        whole &= fresh[k] == 0xffffffffu;
     }
-    if (fresh || (grew && old)) {
+    if (any_fresh || (grew && any_old)) {
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             uint4* pc = reinterpret_cast<uint4*>(code + c * 512);
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-            if (gap) {
+            const float* v = val[c];
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                w[k] = V ? encode4<E4M3>(__fmul_rn(v[k], inv), __fmul_rn(v[4 + k], inv), __fmul_rn(v[8 + k], inv),
+                                         __fmul_rn(v[12 + k], inv))
+                         : encode4<E4M3>(__fmul_rn(v[4 * k], inv), __fmul_rn(v[4 * k + 1], inv),
+                                         __fmul_rn(v[4 * k + 2], inv), __fmul_rn(v[4 * k + 3], inv));
+            if (!whole) {
                 const uint4 q = *pc;
-                w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
-            }
+                const uint32_t was[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int p = piece_pos<V>(lane, i) - first;
-                if (p >= 0 && p < m) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) piece_set<V>(w, i, j, encode8<E4M3>(__fmul_rn(val[c][4 * i + j], inv)));
-                } else if (p < 0 && grew) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        piece_set<V>(w, i, j, encode8<E4M3>(__fmul_rn(decode8<E4M3>(piece_get<V>(w, i, j)), ratio)));
+                for (int k = 0; k < 4; k++) {
+                    uint32_t x = was[k];
+                    if (grew && old[k]) {
+                        float f[4];
+                        decode4<E4M3>(x, f);
+                        x = encode4<E4M3>(__fmul_rn(f[0], ratio), __fmul_rn(f[1], ratio), __fmul_rn(f[2], ratio),
+                                          __fmul_rn(f[3], ratio));
+                        x = (x & old[k]) | (was[k] & ~old[k]);
+                    }
+                    w[k] = (w[k] & fresh[k]) | (x & ~fresh[k]);
                 }
             }
             *pc = make_uint4(w[0], w[1], w[2], w[3]);
@@ -434,13 +448,16 @@ __device__ __forceinline__ void gather_block(const uint8_t* code, float s, void*
     for (int c = 0; c < HD / 32; c++) {
         const uint4 q = *reinterpret_cast<const uint4*>(code + c * 512);
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        float v[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) decode4<E4M3>(w[k], v[k]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int p = piece_pos<V>(lane, i);
             if (p >= m) continue;
             float f[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) f[j] = __fmul_rn(decode8<E4M3>(piece_get<V>(w, i, j)), s);
+            for (int j = 0; j < 4; j++) f[j] = __fmul_rn(V ? v[j][i] : v[i][j], s);
             store4<DT>(out, at + (size_t)p * ld + c * 32 + piece_dim<V>(lane, i), vec, f);
         }
     }
