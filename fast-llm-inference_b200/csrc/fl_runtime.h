@@ -19,6 +19,10 @@ int cuda_error(cudaError_t e, const char* what);
 // Library stream of the current device (created on first use).
 cudaStream_t device_stream();
 int ensure_device();
+// FL_OK when p is memory that kernels of the current device can read as their
+// own: device memory of that device (or managed memory). FL_E_INVAL for host
+// memory, FL_E_STATE for another device's.
+int check_device_ptr(const void* p, const char* what);
 
 // Device mirror of a dequantized_tensor_t (stored in its `dev` field).
 struct DevTensor {

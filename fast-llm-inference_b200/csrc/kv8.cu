@@ -694,6 +694,8 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     if (!ctx_len || !new_len) return set_error(FL_E_INVAL, "kv8_plan: NULL lengths");
     if (nseq < 1 || nseq > h->c.max_seqs) return set_error(FL_E_INVAL, "kv8_plan: nseq must be 1 .. max_seqs");
     if (max_new < 1) return set_error(FL_E_INVAL, "kv8_plan: max_new must be at least 1");
+    FL_CHECK(check_device_ptr(ctx_len, "kv8_plan: ctx_len"));
+    FL_CHECK(check_device_ptr(new_len, "kv8_plan: new_len"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
     PlanArgs a = {};
     a.ctx = ctx_len;
@@ -735,6 +737,8 @@ FL_API int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, i
     if (rows > 1 && (ldk < w || ldv < w)) return set_error(FL_E_INVAL, "kv8_append: a row stride is below kv_heads * head_dim");
     const int es = elem_size(h->c.dtype);
     if ((uintptr_t)k % es || (uintptr_t)v % es) return set_error(FL_E_INVAL, "kv8_append: rows are not aligned to their type");
+    FL_CHECK(check_device_ptr(k, "kv8_append: k"));
+    FL_CHECK(check_device_ptr(v, "kv8_append: v"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
     AppendArgs a = {};
     a.t = h->t;
@@ -762,6 +766,8 @@ FL_API int fl_kv8_gather(fl_kv8_t* h, int layer, void* k, void* v, int keys, voi
     if (!k || !v) return set_error(FL_E_INVAL, "kv8_gather: NULL outputs");
     const int es = elem_size(h->c.dtype);
     if ((uintptr_t)k % es || (uintptr_t)v % es) return set_error(FL_E_INVAL, "kv8_gather: outputs are not aligned to their type");
+    FL_CHECK(check_device_ptr(k, "kv8_gather: k"));
+    FL_CHECK(check_device_ptr(v, "kv8_gather: v"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
     GatherArgs a = {};
     a.t = h->t;
@@ -794,6 +800,8 @@ FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, in
     if ((uintptr_t)q % es || (uintptr_t)out % es)
         return set_error(FL_E_INVAL, "kv8_attention: rows are not aligned to their type");
     if (mask && ldm < h->max_new) return set_error(FL_E_INVAL, "kv8_attention: mask rows are shorter than max_new");
+    FL_CHECK(check_device_ptr(q, "kv8_attention: q"));
+    FL_CHECK(check_device_ptr(out, "kv8_attention: out"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
     Kv8AttnParams p = {};
     p.k = h->k[layer];

@@ -46,6 +46,18 @@ int ensure_device() {
     return FL_OK;
 }
 
+int check_device_ptr(const void* p, const char* what) {
+    FL_CHECK(ensure_device());
+    int dev = 0;
+    cudaPointerAttributes a = {};
+    FL_CHECK_CUDA(cudaGetDevice(&dev));
+    FL_CHECK_CUDA(cudaPointerGetAttributes(&a, p));
+    if (a.type == cudaMemoryTypeManaged) return FL_OK;
+    if (a.type != cudaMemoryTypeDevice) return set_error(FL_E_INVAL, std::string(what) + " is not device memory");
+    if (a.device != dev) return set_error(FL_E_STATE, std::string(what) + " lives on another device than the current one");
+    return FL_OK;
+}
+
 cudaStream_t device_stream() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;

@@ -162,9 +162,13 @@ int fl_cuda_block_dots_i8_noalloc(const float* A, const dequantized_tensor_t* B,
  * append, attention and gather of a step are ordered by the caller's stream,
  * and captured graphs of one handle must not run at the same time. The calls
  * allocate nothing and can be captured; fl_kv8_plan re-reads the lengths at
- * every replay. `stream` NULL is the library's stream; pass cudaStreamLegacy
+ * every replay. The launches of a call are chosen by the bounds (rows, max_new)
+ * that the host knew: a captured attention holds for plans whose max_new is no
+ * larger than at its capture, a captured append or gather for no more sequences.
+ * The attention's waits on the device are bounded; one that gave up leaves
+ * outputs unwritten, and the next fl_cuda_sync returns FL_E_TIMEOUT. `stream` NULL is the library's stream; pass cudaStreamLegacy
  * ((void*)1) for CUDA's default stream. FL_E_STATE when the current device is
- * not the handle's. */
+ * not the handle's, or not that of an array; FL_E_INVAL for host memory. */
 #define FL_F32  0
 #define FL_F16  1
 #define FL_BF16 2

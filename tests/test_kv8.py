@@ -541,6 +541,12 @@ def test_gpu_refusals(gpu):
     q3 = torch.zeros((3, 4, 64), device="cuda")
     with pytest.raises(flb200.FLError, match="shorter than max_new"):
         p.c.attention(0, q3, q3.clone(), mask=torch.ones((3, 3), dtype=torch.uint8, device="cuda"))
+    host = np.zeros(4096, np.float32)
+    for rc in (gpu.fl_kv8_append(p.c.h, 0, flb200.ptr(host), flb200.ptr(host), 1, 128, 128, None),
+               gpu.fl_kv8_attention(p.c.h, 0, q.data_ptr(), flb200.ptr(host), 1, 256, 256, 1.0, None, 0, None),
+               gpu.fl_kv8_gather(p.c.h, 0, flb200.ptr(host), flb200.ptr(host), 1, None),
+               gpu.fl_kv8_plan(p.c.h, flb200.ptr(host), flb200.ptr(host), 1, 1, None)):
+        assert rc == -1 and "not device memory" in gpu.err()
     p.c.append(1, k[:0], k[:0])     # nothing is nothing
     p.c.attention(1, q[:0], q[:0])
 

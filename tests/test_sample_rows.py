@@ -100,6 +100,30 @@ def test_parameters(gpu, orc, dtype, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [9000, 32064])
+def test_many_rows(gpu, orc, dtype, V):
+    """More rows than the GPU holds at four CTAs a row: one CTA each."""
+    rng = np.random.default_rng(V)
+    R = 160
+    l = make(rng, R, V, dtype)
+    check(gpu, orc, l, rng.random(R), rng.uniform(0.3, 1.5, R), rng.integers(0, 60, R), rng.uniform(0.2, 1.1, R),
+          rng.uniform(0, 0.05, R))
+
+
+@pytest.mark.gpu
+def test_host_memory_is_refused(gpu):
+    import torch
+    l = torch.zeros((2, 100), device="cuda")
+    t = torch.zeros(2, dtype=torch.int32, device="cuda")
+    host = np.zeros((2, 100), np.float32)
+    f = gpu.fl_cuda_sample
+    assert f(flb200.ptr(host), 0, 100, 2, 100, None, None, None, None, l.data_ptr(), t.data_ptr(), None) == -1
+    assert "not device memory" in gpu.err()
+    assert f(l.data_ptr(), 0, 100, 2, 100, None, None, None, None, l.data_ptr(), flb200.ptr(host), None) == -1
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [32760, 32761, 65520, 65521, 131072, 262000])
 def test_clusters(gpu, orc, V):
     rng = np.random.default_rng(V)
