@@ -433,6 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if constexpr (F32) tmem_st8(sb + 32 * w + 16 + 8 * c, lo);
                     }
                 }
+                // the page before is done with, usually long ago: no thread falls two phases
+                // of pv_done behind, which its parity could not tell apart
+                if (j > 0 && !warp_wait(&bar.pv_done, (J - 1) & 1)) { ok = false; break; }
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();

@@ -662,3 +662,28 @@ def test_serving_steps(gpu, orc):
             assert int(tok[r]) == expect(orc, l[r], np.float32(1), 0, np.float32(0.9), np.float32(0), hu[r])
         pos = pos + np.maximum(new, 0)
         pos[1] = max(0, pos[1] - step % 3)          # rejected drafts of one sequence
+
+
+def cold_attention():
+    """The first launches of a process: kernels still without their instructions
+    in the caches, so that the warps of a CTA run far apart. (For a child process.)"""
+    lib = flb200.Lib()
+    lib.check(lib.fl_cuda_init(0), "init")
+    rng = np.random.default_rng(12)
+    p = Pair(lib, pages=24, max_seqs=4, max_rows=300, max_ctx=400)
+    for ctx, new in (([0] * 4, [37, 0, 64, 0]), ([37, 0, 64, 0], [1, 100, 1, 0])):
+        p.plan(ctx, new)
+        p.append(p.rows(rng, 2, scale=2.0), p.rows(rng, 2))
+        p.check_attention(p.rows(rng, 4))
+    lib.check(lib.fl_cuda_sync(), "sync")
+
+
+@pytest.mark.gpu
+def test_first_launches_of_a_process(gpu):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = f"import sys; sys.path[:0] = {[here, os.path.dirname(flb200.LIB_PATH)]!r}; import test_kv8; test_kv8.cold_attention()"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
