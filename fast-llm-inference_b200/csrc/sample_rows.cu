@@ -44,6 +44,7 @@ struct SampleArgs {
     const void* logits;
     size_t ld;
     int V, seg;                   // tokens of a CTA of the row's cluster
+    int rows, ahead;              // rows; how many later the row that an SM takes next
     const float *temperature, *top_p, *min_p, *u;
     const int* top_k;
     int* tokens;
@@ -254,13 +255,22 @@ __global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kern
     R row(shared);
     const int r = blockIdx.x / CL;
     const char* l = static_cast<const char*>(a.logits) + (size_t)r * a.ld * ES;
-    const int i0 = row.rank * a.seg, i1 = min(a.V, i0 + a.seg);   // this CTA's tokens
+    const int V = a.V;
+    const int i0 = row.rank * a.seg, i1 = min(V, i0 + a.seg);   // this CTA's tokens
     // token of (group j, element e) of this thread: a warp's tokens are a
     // contiguous piece, groups of VEC begin on 16-byte boundaries, the first
     // of the CTA at or before token i0
     const int first = i0 - (int)(((uintptr_t)l + (size_t)i0 * ES) % 16) / ES + row.warp * (32 * kTok) + row.lane * VEC;
     auto token = [&](int j, int e) { return first + j * (32 * VEC) + e; };
 
+    // The row that this SM takes next, into L2 while this one is worked on: one CTA
+    // holds the SM's registers, so nothing else overlaps its loads with arithmetic.
+    if (CL == 1 && threadIdx.x == 0 && r + a.ahead < a.rows) {
+        const uintptr_t n0 = (uintptr_t)l + (size_t)a.ahead * a.ld * ES, n1 = n0 + (size_t)V * ES;
+        const uintptr_t p0 = (n0 + 15) & ~(uintptr_t)15, p1 = n1 & ~(uintptr_t)15;
+        if (p1 > p0)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p0), "r"((uint32_t)(p1 - p0)) : "memory");
+    }
     uint32_t w[kTok];   // logits, then weights
     const int w0 = token(0, 0) - row.lane * VEC;   // this warp's tokens
     if (w0 >= i0 && w0 + 32 * kTok <= i1) {
@@ -415,48 +425,80 @@ __global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kern
 
     if (kth && lo == kth) {
         // top-k keeps `room` of the `ties` weights equal to kth: the largest
-        // logits, equal ones in index order (different logits can share a weight)
-        uint32_t top = 0, bot = 0;
+        // logits, equal ones in index order (different logits can share a weight,
+        // far below the maximum thousands of them)
+        constexpr uint32_t kHalf = 0x80000000u, kKept = 1u << 29;
+        const uint32_t tie = kth + kTag;
+        uint32_t top, bot;
+        auto range = [&]() {   // of the ties' keys
+            uint32_t hi = 0, lo_c = 0;
 #pragma unroll
-        for (int j = 0; j < J; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int e = 0; e < VEC; e++)
-                if (w[j * VEC + e] == kth + kTag) {
-                    const uint32_t s = sortable(logit<DT>(l, token(j, e)));
-                    top = max(top, s);
-                    bot = max(bot, ~s);
-                }
-        top = row.max32(top);
-        bot = ~row.max32(bot);
-        auto key_count = [&](uint32_t t) {   // ties with a key of at least t
+                for (int e = 0; e < VEC; e++)
+                    if (w[j * VEC + e] == tie) {
+                        const uint32_t s = sortable(logit<DT>(l, token(j, e)));
+                        hi = max(hi, s);
+                        lo_c = max(lo_c, ~s);
+                    }
+            top = row.max32(hi);
+            bot = ~row.max32(lo_c);
+        };
+        range();
+        u64 left = ties, need = room;
+        if (top - bot >= kHalf) {   // both signs, a vast temperature: the one that the cut lies in
             uint32_t c = 0;
 #pragma unroll
             for (int j = 0; j < J; j++)
 #pragma unroll
                 for (int e = 0; e < VEC; e++)
-                    if (w[j * VEC + e] == kth + kTag) c += sortable(logit<DT>(l, token(j, e))) >= t;
-            return row.sum(0, c);
-        };
-        // bot: the largest key with `room` ties at or above it
-        uint32_t up = top + 1u;
-        u64 above = 0;
-        while (up - bot > 1u) {
-            const uint32_t mid = bot + (up - bot) / 2u;
-            const u64 c = key_count(mid);
-            if (c >= room) bot = mid; else { up = mid; above = c; }
+                    if (w[j * VEC + e] == tie) c += sortable(logit<DT>(l, token(j, e))) >= kHalf;
+            const u64 pos = row.sum(0, c);
+            const bool up = pos >= need;
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    if (w[j * VEC + e] == tie && (sortable(logit<DT>(l, token(j, e))) >= kHalf) != up)
+                        w[j * VEC + e] = up ? kTag : tie | kKept;   // dropped, or kept without more ado
+            left = up ? pos : left - pos;
+            need = up ? need : need - pos;
+            range();
         }
-        auto equal = [&](uint32_t& sum, int i, int n, uint32_t t) {
-            if (w[i] == t) sum += sortable(logit<DT>(l, n)) == bot;
-        };
-        const uint32_t last = locate(kth + kTag, equal, [&](u64) { return room - above - 1; }, true);
+        if (need < left) {
+            // the ties as their keys less the smallest, below 2^31, marked by the top bit
 #pragma unroll
-        for (int j = 0; j < J; j++)
+            for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int e = 0; e < VEC; e++)
-                if (w[j * VEC + e] == kth + kTag) {
-                    const uint32_t s = sortable(logit<DT>(l, token(j, e)));
-                    if (s < bot || (s == bot && (uint32_t)token(j, e) > last)) w[j * VEC + e] = kTag;
+                for (int e = 0; e < VEC; e++)
+                    if (w[j * VEC + e] == tie)
+                        w[j * VEC + e] = kHalf + (sortable(logit<DT>(l, token(j, e))) - bot);
+            // cut: as many keys at or above it as are needed, or the largest with at least as many
+            uint32_t cut = kHalf, end = kHalf + (top - bot) + 1u;
+            u64 at_cut = left, at_end = 0;
+            while (end - cut > 1u && at_cut != need) {
+                const uint32_t mid = cut + (end - cut) / 2u;
+                uint32_t c = 0;
+#pragma unroll
+                for (int i = 0; i < kTok; i++) c += w[i] >= mid;
+                const u64 n = row.sum(0, c);
+                if (n >= need) { cut = mid; at_cut = n; } else { end = mid; at_end = n; }
+            }
+            uint32_t last = 0xffffffffu;   // of the tokens at the cut, the last one kept
+            if (at_cut != need)
+                last = locate(cut, [&](uint32_t& sum, int i, int, uint32_t t) { sum += w[i] == t; },
+                              [&](u64) { return need - at_end - 1; }, true);
+#pragma unroll
+            for (int j = 0; j < J; j++)
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    const uint32_t x = w[j * VEC + e];
+                    if (x >= kHalf)
+                        w[j * VEC + e] = x > cut || (x == cut && (uint32_t)token(j, e) <= last) ? tie : kTag;
                 }
+        }
+#pragma unroll
+        for (int i = 0; i < kTok; i++) w[i] &= ~kKept;
     }
     const uint32_t U = min(fixed24(a.u[r]), kOne - 1u);
     locate(lo + kTag, [&](uint32_t& sum, int i, int, uint32_t t) { add_if_ge(sum, w[i], t, row.one); },
@@ -499,10 +541,12 @@ cudaError_t sample_dt(SampleArgs a, int rows, cudaStream_t s) {
         a.seg = ((a.V + cl - 1) / cl + 7) / 8 * 8;
         return a.seg <= cta_tokens(threads);
     };
+    a.ahead = 4 * sample_sms();
     if (fits(128, 1)) return launch_sample<DT, 128, 1>(a, rows, s);
     // while all CTAs of four to a row are resident (several share an SM): one row of
     // 32064 took 17 us in four CTAs of 128 threads, 20 in one of 512
     if (rows * 4 <= sample_sms() * 2 && fits(128, 4)) return launch_sample<DT, 128, 4>(a, rows, s);
+    a.ahead = sample_sms();
     if (fits(512, 1)) return launch_sample<DT, 512, 1>(a, rows, s);
     if (fits(256, 8)) return launch_sample<DT, 256, 8>(a, rows, s);
     if (fits(512, 8)) return launch_sample<DT, 512, 8>(a, rows, s);
@@ -530,7 +574,7 @@ FL_API int fl_cuda_sample(const void* logits, int dtype, size_t ld, int rows, in
     FL_CHECK(check_device_ptr(logits, "sample: logits"));
     FL_CHECK(check_device_ptr(tokens, "sample: tokens"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
-    const SampleArgs a = {logits, ld, V, 0, temperature, top_p, min_p, u, top_k, tokens};
+    const SampleArgs a = {logits, ld, V, 0, rows, 0, temperature, top_p, min_p, u, top_k, tokens};
     FL_CHECK_CUDA(dtype == FL_F32 ? sample_dt<FL_F32>(a, rows, s)
                                   : dtype == FL_F16 ? sample_dt<FL_F16>(a, rows, s) : sample_dt<FL_BF16>(a, rows, s));
     return FL_OK;

@@ -151,6 +151,20 @@ def test_ties(gpu, orc, dtype, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("V", [500, 32064])
+def test_logits_that_share_a_weight(gpu, orc, dtype, V):
+    """Temperatures at which many different logits have the weight of the k-th:
+    far below the maximum, or so hot that all are equal (keys of both signs)."""
+    rng = np.random.default_rng(V)
+    l = make(rng, 6, V, dtype, 2.0)
+    l[:, 7] = 20.0
+    for k in (1, 2, 40, V // 2, V - 1):
+        check(gpu, orc, l, rng.random(6), [1.15, 0.9, 1e9, 1e15, 1e25, np.inf], [k] * 6, None, None)
+        check(gpu, orc, l, rng.random(6), [1.15, 1e9, 1e9, 1e25, 1.0, 0.8], [k] * 6, [0.9999] * 6, None)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [5, 3000, 33000])
 def test_special_values(gpu, orc, V):
     import torch
