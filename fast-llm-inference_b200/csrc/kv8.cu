@@ -22,7 +22,8 @@ namespace {
 // return and take pages and write the row maps, item by item: an item's sequence
 // is found by bisection in the starts, which lie in shared memory up to
 // 1024 sequences. Bound by latency: the loads of the lengths, two barriers of the scan, the
-// page loads and stores with a barrier after each.
+// page loads and stores with a barrier after each: 5.4 us for 8 sequences of one row;
+// 32 us each to drop and to admit 1021 sequences with 33 k pages and 40 k rows.
 // ---------------------------------------------------------------------------
 constexpr int kSmSeqs = 1024;   // sequences whose starts shared memory holds
 
@@ -288,7 +289,8 @@ __global__ void kv8_reset_kernel(const Kv8Tables t, int pages, int max_seqs) {
 // holds the 16 codes of its 16 stored bytes per chunk of 32 dimensions (see
 // fl_kv8.h), so the block's largest value is one warp reduction, and a stored
 // piece is read, recoded where the scale grew, filled in and written whole.
-// Bound by bytes: the rows once in, the codes once out.
+// Bound by bytes: the rows once in, the codes once out; with the gather behind it
+// 14 k bf16 rows of 10 x 128 take 77 us, the bytes of both 40.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     Kv8Tables t;
@@ -431,7 +433,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) kv8_append_kernel(const App
 // ---------------------------------------------------------------------------
 // Gather: the values that the codes of every planned sequence stand for,
 // packed [key][kv head][head_dim]. One warp per (16-position block, kv head,
-// K or V); bound by the bytes written.
+// K or V); bound by the bytes written, at few blocks by the chain of loads before
+// them (the block's sequence, page and scale).
 // ---------------------------------------------------------------------------
 struct GatherArgs {
     Kv8Tables t;

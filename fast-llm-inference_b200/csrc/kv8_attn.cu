@@ -8,7 +8,7 @@
 // block's power-of-two scales multiply its scores, and its probabilities,
 // exactly. Rows of 8 dimensions and of 4 positions lie in the cache in the
 // products' operand order, so a warp reads a block of 16 positions with one
-// 16-byte load per lane and 32 dimensions, straight into registers.
+// 16-byte copy per lane and 32 dimensions, through its own slots in shared memory.
 //
 // Queries enter as halves too, each row shifted by a power of two so that its
 // largest value lies in [2^14, 2^15): exact for fp16 and bf16 rows down to
@@ -16,6 +16,12 @@
 // remainder, 22 bits together): a tile then holds 8 rows, their remainders in
 // the tile's other 8 rows, so the second half costs no further product. The
 // probabilities of f32 rows are split the same way.
+//
+// Bound by the cache's bytes: 24 rows over 300 to 32000 keys (40 / 10 heads of 128,
+// 0.91 GB) take 169 us, 5.4 TB/s or 83 % of the copy peak; 64 x 7 rows over 1000 to
+// 1500 keys (32 heads of 96, 0.53 GB) 111 us, 73 %. Loads straight into registers
+// took 315 and 142 us: a warp waited for each block. Each warp takes one block of
+// every page, so that nothing is shared before the tile's end.
 #include <math.h>
 
 #include <algorithm>

@@ -13,8 +13,10 @@
 // The draw is a prefix sum in token order: over the warps, each of which holds
 // a contiguous piece of the row, then within the one the target falls into.
 // Bound by instructions: about 25 a token for its weight, 3 for each of about
-// eight passes; few warps with much work each, because what a pass costs apart
-// from that are the warps' reductions.
+// nine passes a threshold; few warps with much work each, because what a pass costs
+// apart from that are the warps' reductions (32 tokens a thread of 1024 took 85 us
+// where this takes 74: 448 rows of 32064 with mixed rules). One row takes 17 us, 61
+// rows of 128011 in 16 bits 112.
 #include <float.h>
 #include <limits.h>
 
