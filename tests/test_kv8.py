@@ -359,10 +359,10 @@ def test_strided_and_short_rows(gpu, dtype):
     behind the planned ones, and planned ones behind the buffer, are left alone."""
     rng = np.random.default_rng(4)
     H, Hk, hd = 4, 2, 64
-    for pad in (0, 1, 8):
+    for pad, new in ((0, 30), (1, 30), (8, 30), (0, 99), (1, 99)):
         p = Pair(gpu, heads=H, kv_heads=Hk, hd=hd, dtype=dtype)
-        p.plan([0, 0], [21, 30])
-        T = 51
+        p.plan([0, 0], [21, new])
+        T = 21 + new
         w = (H + 2 * Hk) * hd + pad
         buf = dev(rng.standard_normal((T + 6) * w + 16), torch.float32).to(getattr(torch, dtype))
         at = lambda off, heads: buf.as_strided((T + 6, heads, hd), (w, hd, 1), off)
@@ -392,6 +392,8 @@ FORMS = [
     (4, 1, 128, [130, 0, 1], [70, 129, 33]),
     (14, 2, 96, [0, 61], [61, 20]),
     (6, 2, 32, [900], [150]),
+    (2, 2, 64, [500, 0], [200, 193]),
+    (8, 1, 96, [33, 70], [24, 33]),
 ]
 
 
@@ -460,7 +462,7 @@ def test_positions_behind_the_sequence_do_not_matter(gpu, type):
     """Recycled pages full of the largest codes behind the last position, and
     rolled-back rows with other scales."""
     rng = np.random.default_rng(7)
-    for nb in (1, 60):
+    for nb in (1, 60, 110):
         p = Pair(gpu, heads=2, kv_heads=1, hd=64, dtype="float16", type=type, pages=6, max_seqs=2, max_ctx=384)
         p.plan([0], [384])
         big = torch.full((384, 1, 64), 60000.0, dtype=torch.float16, device="cuda")
@@ -481,7 +483,7 @@ def test_positions_behind_the_sequence_do_not_matter(gpu, type):
 def test_rows_stand_alone(gpu):
     """A NaN in one query row, or an infinity, stays in that row and head."""
     rng = np.random.default_rng(8)
-    for new in (3, 80):
+    for new in (3, 80, 100):
         p = Pair(gpu, heads=2, kv_heads=1, hd=64)
         p.plan([0], [50])
         p.append(p.rows(rng, 1), p.rows(rng, 1))
