@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
     extern __shared__ __align__(128) uint8_t smem[];   // rings of the warps, then their results
     float(*o_s)[TR][HD] = reinterpret_cast<float(*)[TR][HD]>(smem);
     __shared__ float m_s[kAW][TR], l_s[kAW][TR];
-    __shared__ int last_s;
+    __shared__ Kv8Joins joins;
+    if (threadIdx.x == 0) joins.n = 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * kStage);
     const int g = lane >> 2, t4 = lane & 3;
@@ -349,27 +350,19 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                 if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
             }
         }
-        if (it.splits > 1) {
-            // the last range to arrive joins the tile's ranges, in their order
-            int* cnt = tl.part_cnt + it.part;
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) last_s = atomicAdd(cnt, 1) == it.splits - 1;
-            __syncthreads();
-            if (last_s) {
-                __threadfence();
-                for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kAW * 32) {
-                    const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
-                    float acc[4];
-                    join_parts(tl, it, TR, HD, r, d, acc);
-                    const int pr = it.tile * TR + r, tk = pr / p.group;
-                    const int hq = h * p.group + pr - tk * p.group;
-                    if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
-                }
-                if (threadIdx.x == 0) *cnt = 0;
-            }
-        }
+        if (it.splits > 1) range_done(tl, it, joins);
         __syncthreads();
+    }
+    // the tiles that this CTA completed, each from its ranges in their order
+    __threadfence();
+    for (int k = 0; k < joins.n; k++) {
+        const Kv8Item& jt = joins.item[k];
+        join_tile<HD, kAW * 32>(tl, jt, TR, min(TR, jt.nb * p.group - jt.tile * TR), [&](int r, int d, const float (&acc)[4]) {
+            const int pr = jt.tile * TR + r, tk = pr / p.group;
+            const int hq = jt.head * p.group + pr - tk * p.group;
+            if (jt.row0 + tk < p.rows)
+                store4<DT>(p.out, (size_t)(jt.row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
+        });
     }
 }
 

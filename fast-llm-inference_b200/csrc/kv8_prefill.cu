@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(8) TileBars bars[2];
     __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     __shared__ uint32_t tmem_s;
-    __shared__ int bad_s, last_s;
+    __shared__ int bad_s;
+    __shared__ Kv8Joins joins;
     __shared__ Kv8Item it;
     const uint32_t smem = (saddr(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mb_init(&v_full[i], 4);
             mb_init(&v_empty[i], 1);
         }
-        bad_s = 0;
+        bad_s = joins.n = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -623,32 +624,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             jt1 += n;
             items1 += n > 0;
         }
-        if (it.splits > 1) {
-            // the last range to arrive joins the tile's ranges, in their order
-            int* cnt = tl.part_cnt + it.part;
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) last_s = atomicAdd(cnt, 1) == it.splits - 1;
-            __syncthreads();
-            if (last_s) {
-                __threadfence();
-                for (int idx = threadIdx.x; idx < np * (HD / 4); idx += kThreads) {
-                    const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
-                    float acc[4];
-                    join_parts(tl, it, kPair, HD, r, d, acc);
-                    const int pr = it.tile * kPair + r, tk = pr / p.group;
-                    const int hq = h * p.group + pr - tk * p.group;
-                    if (row0 + tk < p.rows) store4<DT>(p.out, (size_t)(row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
-                }
-                if (threadIdx.x == 0) *cnt = 0;
-            }
-        }
+        if (it.splits > 1) range_done(tl, it, joins);
         __syncthreads();
     }
     __syncthreads();
     if (warp == 12) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+    // the tiles that this CTA completed, each from its ranges in their order
+    __threadfence();
+    for (int k = 0; k < joins.n && !bad_s; k++) {
+        const Kv8Item& jt = joins.item[k];
+        join_tile<HD, kThreads>(tl, jt, kPair, min(kPair, jt.nb * p.group - jt.tile * kPair), [&](int r, int d, const float (&acc)[4]) {
+            const int pr = jt.tile * kPair + r, tk = pr / p.group;
+            const int hq = jt.head * p.group + pr - tk * p.group;
+            if (jt.row0 + tk < p.rows)
+                store4<DT>(p.out, (size_t)(jt.row0 + tk) * p.ldo + (size_t)hq * HD + d, vec, acc);
+        });
     }
 }
 
