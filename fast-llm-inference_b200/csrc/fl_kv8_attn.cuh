@@ -96,7 +96,9 @@ __device__ __forceinline__ void next_item(const Kv8AttnParams& p, const Kv8Tiles
     const bool whole = ceilf(per_cta) * (mean + kTileCost) + ((float)mt.list[tl.list].max_pages - mean) <=
                        per_cta * mean + (per_cta + 1.0f) * kTileCost + kJoinCost;
     const long long total = (whole ? tiles : work) * p.kv_heads;
-    const long long size = whole ? 1 : (total + G - 1) / G;
+    // a prefill part of n pages takes about 2 n us, and its share of a join 1.3
+    const int least = tl.list ? (int)ceilf(sqrtf(0.65f * mean)) : 1;
+    const long long size = whole ? 1 : max((long long)least, (total + G - 1) / G);
     if (x < 0) x = (long long)blockIdx.x * size;
     Kv8Item it = {};
     if (x < (whole ? total : min(total, (blockIdx.x + 1ll) * size))) {
@@ -153,34 +155,40 @@ __device__ __forceinline__ void range_done(const Kv8Tiles& tl, const Kv8Item& it
 }
 
 // Rows 0 .. np - 1 of a tile joined from its parts' results, in the parts' order,
-// by a block of NT threads; put(row, dimension, four values). First a warp a
-// row turns (m, l) into the parts' weights l 2^(m - M) and the row's 1 / sum, in
+// by a block of NT threads; put(row, dimension, four values). First some lanes
+// a row turn (m, l) into the parts' weights l 2^(m - M) and the row's 1 / sum, in
 // place (the last to arrive is alone with them); then the loads of the results do not
 // wait on each other. Weights within the loop over the results, one load
 // behind the other, made the join the longest part of a call over few tiles: 256
 // rows x 10 heads over 16 k keys took 301 us.
-template <int HD, int NT, class Put>
-__device__ __forceinline__ void join_tile(const Kv8Tiles& tl, const Kv8Item& it, int rows, int np, Put put) {
+template <int HD, int NT, int ROWS, class Put>
+__device__ __forceinline__ void join_tile(const Kv8Tiles& tl, const Kv8Item& it, int np, Put put) {
     constexpr int U = 8;   // results under way
-    const int lane = threadIdx.x & 31;
+    constexpr int GL = NT / ROWS >= 16 ? 16 : NT / ROWS >= 8 ? 8 : 1;   // lanes of a row
+    static_assert(NT >= GL * ROWS, "a row for every group of lanes");
     // slots of a part: its first range, of a tile begun before it, and its last
-    auto at = [&](int k, int r) { return (2 * (size_t)(it.part + k) + (k == 0)) * rows + r; };
-    for (int r = threadIdx.x >> 5; r < np; r += NT / 32) {
-        float M = -INFINITY, L = 0.0f;
-        for (int k = lane; k < it.splits; k += 32) M = fmaxf(M, __ldcg(&tl.part_ml[at(k, r)]).x);
+    auto at = [&](int k, int r) { return (2 * (size_t)(it.part + k) + (k == 0)) * ROWS + r; };
+    const int row = threadIdx.x / GL, first = row < np ? (int)threadIdx.x % GL : it.splits;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+    for (int k = first; k < it.splits; k += GL) M = fmaxf(M, __ldcg(&tl.part_ml[at(k, row)]).x);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        for (int k = lane; k < it.splits; k += 32) {
-            const float2 ml = __ldcg(&tl.part_ml[at(k, r)]);
-            const float w = ml.y != 0.0f ? ml.y * ex2(ml.x - M) : 0.0f;   // NaN sums stay NaN
+    for (int o = GL / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int k0 = first; k0 < it.splits; k0 += 4 * GL) {
+        float2 ml[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            ml[u] = k0 + u * GL < it.splits ? __ldcg(&tl.part_ml[at(k0 + u * GL, row)]) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float w = ml[u].y != 0.0f ? ml[u].y * ex2(ml[u].x - M) : 0.0f;   // NaN sums stay NaN
             L += w;
-            tl.part_ml[at(k, r)].x = w;
+            if (k0 + u * GL < it.splits) tl.part_ml[at(k0 + u * GL, row)].x = w;
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        const float f = L != 0.0f ? __fdiv_rn(1.0f, L) : 0.0f;
-        for (int k = lane; k < it.splits; k += 32) tl.part_ml[at(k, r)].y = f;
     }
+#pragma unroll
+    for (int o = GL / 2; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (first == 0 && row < np) tl.part_ml[at(0, row)].y = L != 0.0f ? __fdiv_rn(1.0f, L) : 0.0f;
     __syncthreads();
     for (int idx = threadIdx.x; idx < np * (HD / 4); idx += NT) {
         const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
@@ -196,7 +204,7 @@ __device__ __forceinline__ void join_tile(const Kv8Tiles& tl, const Kv8Item& it,
                     v[u] = __ldcg(reinterpret_cast<const float4*>(tl.part + at(k0 + u, r) * HD + d));
                 }
             }
-            f = wf[0].y;
+            if (k0 == 0) f = wf[0].y;
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 if (wf[u].x == 0.0f) continue;

@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
     __threadfence();
     for (int k = 0; k < joins.n; k++) {
         const Kv8Item& jt = joins.item[k];
-        join_tile<HD, kAW * 32>(tl, jt, TR, min(TR, jt.nb * p.group - jt.tile * TR), [&](int r, int d, const float (&acc)[4]) {
+        join_tile<HD, kAW * 32, TR>(tl, jt, min(TR, jt.nb * p.group - jt.tile * TR), [&](int r, int d, const float (&acc)[4]) {
             const int pr = jt.tile * TR + r, tk = pr / p.group;
             const int hq = jt.head * p.group + pr - tk * p.group;
             if (jt.row0 + tk < p.rows)

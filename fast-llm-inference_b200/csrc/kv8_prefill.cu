@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __threadfence();
     for (int k = 0; k < joins.n && !bad_s; k++) {
         const Kv8Item& jt = joins.item[k];
-        join_tile<HD, kThreads>(tl, jt, kPair, min(kPair, jt.nb * p.group - jt.tile * kPair), [&](int r, int d, const float (&acc)[4]) {
+        join_tile<HD, kThreads, kPair>(tl, jt, min(kPair, jt.nb * p.group - jt.tile * kPair), [&](int r, int d, const float (&acc)[4]) {
             const int pr = jt.tile * kPair + r, tk = pr / p.group;
             const int hq = jt.head * p.group + pr - tk * p.group;
             if (jt.row0 + tk < p.rows)
