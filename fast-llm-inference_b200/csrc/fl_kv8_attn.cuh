@@ -11,7 +11,7 @@
 
 namespace fl {
 
-constexpr float kTileCost = 3.0f, kJoinCost = 20.0f;   // in pages, see the kernel
+constexpr float kTileCost = 3.0f, kJoinCost = 20.0f;   // in pages, see next_item
 constexpr float kShift = 7.0f;   // probabilities enter as 2^7 p: 2^-21 of the largest is a normal half
 constexpr float kSlack = 8.0f;   // the reference follows the maximum once it lags by 2^8
 
@@ -87,7 +87,8 @@ __device__ __forceinline__ int find_work(const long long* start, int nseq, long 
 // together whatever the lengths are, while a tile that several parts share is
 // joined by the last of them to arrive. What each takes is estimated in pages:
 // kTileCost a tile, kJoinCost for the joins. At 64 x 32 tiles of 21 pages whole
-// tiles took 106 us and parts 120; at 24 x 10 tiles of 5 to 500, 290 and 168.
+// tiles took 106 us and parts 120; at 24 x 10 tiles of 5 to 500, 290 and 168; in the
+// prefill kernel at 10 tiles of 11 pages, 45 and 74.
 __device__ __forceinline__ void next_item(const Kv8AttnParams& p, const Kv8Tiles& tl, long long x, int lane,
                                           Kv8Item& out) {
     const Kv8Meta& mt = *p.t.meta;
@@ -160,7 +161,7 @@ __device__ __forceinline__ void range_done(const Kv8Tiles& tl, const Kv8Item& it
 // place (the last to arrive is alone with them); then the loads of the results do not
 // wait on each other. Weights within the loop over the results, one load
 // behind the other, made the join the longest part of a call over few tiles: 256
-// rows x 10 heads over 16 k keys took 301 us.
+// rows x 10 heads over 16 k keys took 301 us, now 128.
 template <int HD, int NT, int ROWS, class Put>
 __device__ __forceinline__ void join_tile(const Kv8Tiles& tl, const Kv8Item& it, int np, Put put) {
     constexpr int U = 8;   // results under way

@@ -28,12 +28,18 @@ namespace {
 constexpr int kSmSeqs = 1024;   // sequences whose starts shared memory holds
 
 // Packed query rows of a sequence (new rows x heads per kv head) from which the
-// prefill kernel takes it: at 132 rows and 3700 keys (4 x 10 heads) it took 110 us,
-// the row kernel 84; at 3200 to 8200 rows 0.83 ms, the row kernel 2.47.
+// prefill kernel takes it. 128 / 188 rows in 16 bits: 4 sequences x 3700 keys (10 kv
+// heads x 128) 71 / 93 us, the row kernel 68 / 94; 1 x 16 k 84 / 112, 69 / 91; 32 x 1000
+// 120 / 157, 155 / 229. f32, whose products are twice as many in either, at 96 rows (32
+// heads x 96): 116, 133 and 309 us, the row kernel 187, 183 and 490; at 64 rows 112, 128
+// and 289 to 129, 128 and 316, but 32 to 15 at one sequence of 600 keys.
 #ifndef FL_KV8_LONG_MIN
 #define FL_KV8_LONG_MIN 192
 #endif
-constexpr int kLongMin = FL_KV8_LONG_MIN;
+#ifndef FL_KV8_LONG_MIN_F32
+#define FL_KV8_LONG_MIN_F32 96
+#endif
+int long_min(const fl_kv8_t* h) { return h->c.dtype == FL_F32 ? FL_KV8_LONG_MIN_F32 : FL_KV8_LONG_MIN; }
 
 struct PlanArgs {
     const int *ctx, *nw;
@@ -716,7 +722,7 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     a.max_rows = h->c.max_rows;
     a.group = h->group;
     a.tile_rows = h->tile_rows;
-    a.long_min = kLongMin;
+    a.long_min = long_min(h);
     // one CTA while its threads hold the rows; eight (a portable cluster) beyond
     const long long rows = std::min<long long>((long long)nseq * a.max_new, h->c.max_rows);
     const bool small = nseq <= 256 && rows <= 1024;
@@ -837,6 +843,6 @@ FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, in
     for (int i = 0; i < 2; i++)
         tl[i] = Kv8Tiles{i, h->t.tile_start[i], h->t.work_start[i], h->part[i], h->part_ml[i], h->part_cnt[i]};
     FL_CHECK_CUDA(launch_kv8_attention(p, tl[0], h->parts[0], s));
-    if ((long long)h->max_new * h->group >= kLongMin) FL_CHECK_CUDA(launch_kv8_prefill(p, tl[1], h->parts[1], s));
+    if ((long long)h->max_new * h->group >= long_min(h)) FL_CHECK_CUDA(launch_kv8_prefill(p, tl[1], h->parts[1], s));
     return FL_OK;
 }
