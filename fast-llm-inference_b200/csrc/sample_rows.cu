@@ -204,7 +204,9 @@ __device__ __forceinline__ uint32_t bisect(R& row, const uint32_t (&w)[kTok], ui
     }
     if (hi - lo <= 1u) return lo;
     // the undecided weights of the whole row in every CTA, each against all of
-    // them: the threshold is the largest at which ok holds
+    // them: the threshold is the largest at which ok holds. A call may come here
+    // without a pass, while other warps still sum the pairs of the call before.
+    __syncthreads();
     for (int i = threadIdx.x; i < kPairs; i += R::NW * 32) row.sm.pairs[i] = 0u;
     if (threadIdx.x == 0) row.sm.n = 0;
     __syncthreads();

@@ -112,6 +112,27 @@ def test_many_rows(gpu, orc, dtype, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R,V", [(160, 8000), (160, 20000), (8, 20000), (24, 60000), (12, 200000)])
+def test_top_p_right_behind_a_small_top_k(gpu, orc, R, V):
+    """At most 128 weights above the k-th: top-p then compares its weights all
+    with all right after top-k did, in the same shared list. In every form
+    (threads of a CTA, CTAs of a row), each call repeated."""
+    import torch
+    rng = np.random.default_rng(V)
+    l = make(rng, R, V, "float32")
+    k = rng.integers(2, 129, R)
+    p = rng.uniform(0.3, 0.99, R)
+    u = rng.random(R)
+    check(gpu, orc, l, u, None, k, p, None)
+    want = run(gpu, l, u, None, k, p)
+    d = [torch.tensor(np.asarray(a), dtype=t, device="cuda") for a, t in ((u, torch.float32), (k, torch.int32), (p, torch.float32))]
+    out = torch.empty((300, R), dtype=torch.int32, device="cuda")
+    for o in out:
+        flb200.sample(gpu, l, d[0], o, None, d[1], d[2], stream=0)
+    assert (out.cpu().numpy() == want).all()
+
+
+@pytest.mark.gpu
 def test_host_memory_is_refused(gpu):
     import torch
     l = torch.zeros((2, 100), device="cuda")
