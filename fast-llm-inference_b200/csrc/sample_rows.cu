@@ -116,6 +116,12 @@ struct Row {
         if (CL > 1) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
         me = rank * NW + warp;
         asm volatile("" : "+r"(one));
+        if (CL > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA has started
+    }
+    // Before the first access to another CTA's shared memory: every CTA of the
+    // cluster has to have started.
+    __device__ __forceinline__ void started() {
+        if constexpr (CL > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     }
     __device__ __forceinline__ void sync() {
         if constexpr (CL > 1)
@@ -303,6 +309,7 @@ __global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kern
     float mx = -INFINITY;   // NaN is never the larger
 #pragma unroll
     for (int i = 0; i < kTok; i++) mx = fmaxf(mx, __uint_as_float(w[i]));
+    row.started();
     mx = unsortable(row.max32(sortable(mx)));
     if (mx == INFINITY) {
         mx = FLT_MAX;

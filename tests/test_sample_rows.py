@@ -133,6 +133,27 @@ def test_top_p_right_behind_a_small_top_k(gpu, orc, R, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [9000, 100000, 200000])
+def test_clusters_that_start_one_after_another(gpu, orc, V):
+    """More clusters than the GPU holds, on two streams at once: the CTAs of a
+    row start whenever SMs fall free, next to other rows' ends."""
+    import torch
+    rng = np.random.default_rng(V)
+    R = 70
+    l = make(rng, R, V, "bfloat16")
+    u = torch.tensor(rng.random(R), dtype=torch.float32, device="cuda")
+    out = torch.empty((40, R), dtype=torch.int32, device="cuda")
+    s = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(out):
+        flb200.sample(gpu, l, u, o, stream=s[i % 2].cuda_stream)
+    torch.cuda.synchronize()
+    h, hu = l.float().cpu().numpy(), u.cpu().numpy()
+    want = [expect(orc, h[r], 1.0, 0, np.float32(1), np.float32(0), hu[r]) for r in range(R)]
+    assert (out.cpu().numpy() == want).all()
+
+
+@pytest.mark.gpu
 def test_host_memory_is_refused(gpu):
     import torch
     l = torch.zeros((2, 100), device="cuda")
