@@ -41,6 +41,10 @@ constexpr int kPairs = 128;       // undecided weights compared all with all
 constexpr uint32_t kTag = 1u << 28;
 constexpr int kMassBits = 44;
 constexpr u64 kMass = (1ull << kMassBits) - 1;
+// The weight of a larger logit is smaller, by one, for 2878 of all floats below 0
+// (each against the float before it), with weights from kUnorderedMin to kUnorderedMax:
+// the polynomial's last roundings. tests/sample_weight_check.c goes through all floats.
+constexpr uint32_t kUnorderedMin = 13066122u, kUnorderedMax = 16518617u;
 
 struct SampleArgs {
     const void* logits;
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kern
     // token of (group j, element e) of this thread: a warp's tokens are a
     // contiguous piece, groups of VEC begin on 16-byte boundaries, the first
     // of the CTA at or before token i0
-    const int first = i0 - (int)(((uintptr_t)l + (size_t)i0 * ES) % 16) / ES + row.warp * (32 * kTok) + row.lane * VEC;
+    int first = i0 - (int)(((uintptr_t)l + (size_t)i0 * ES) % 16) / ES + row.warp * (32 * kTok) + row.lane * VEC;
     auto token = [&](int j, int e) { return first + j * (32 * VEC) + e; };
 
     // The row that this SM takes next, into L2 while this one is worked on: one CTA
@@ -329,50 +333,6 @@ __global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kern
         if (row.rank == 0 && threadIdx.x == 0) a.tokens[r] = mx == -INFINITY ? -1 : (int)~best;
         return;
     }
-    // x / T rounded to nearest from one reciprocal (Markstein: with r the
-    // rounded 1 / T, q = x r corrected by r (x - q T) is the rounded quotient
-    // unless T's fraction is all ones), where neither it nor a quotient that
-    // gives a weight leaves the normal range; quotients beyond -17 give 0
-    const uint32_t tb = __float_as_uint(T);
-    if (T > 1e-20f && T < 1e20f && (tb & 0x7fffffu) != 0x7fffffu) {
-        const float rt = __frcp_rn(T), low = -18.0f * T;
-#pragma unroll
-        for (int i = 0; i < kTok; i++) {
-            const float x = __fsub_rn(__uint_as_float(w[i]), mx);
-            const float xc = fmaxf(x, low);   // its weight is 0 too, and its quotient in range
-            const float q0 = __fmul_rn(xc, rt);
-            w[i] = sample_weight(__fmaf_rn(__fmaf_rn(-q0, T, xc), rt, q0)) + kTag;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kTok; i++) w[i] = sample_weight(__fdiv_rn(__fsub_rn(__uint_as_float(w[i]), mx), T)) + kTag;
-    }
-    const u64 all = at_least(row, w, 1u);
-    u64 slo = all, shi = 0;
-    uint32_t lo = 1u;          // kept: the weights >= lo
-    u64 z = all & kMass;
-    const int k = a.top_k ? a.top_k[r] : 0;
-    u64 ties = 0, room = 0;    // weights equal to lo, and how many of them top-k keeps
-    if (k > 0 && (u64)k < (all >> kMassBits)) {
-        lo = bisect(row, w, 1u, kOne + 1u, slo, shi, [&](u64 s) { return (s >> kMassBits) >= (u64)k; });
-        ties = (slo - shi) >> kMassBits;
-        room = (u64)k - (shi >> kMassBits);
-        z = (shi & kMass) + room * lo;
-    }
-    const uint32_t kth = ties > room ? lo : 0u;   // the weight of which only some are kept
-    const float tp = a.top_p ? a.top_p[r] : 1.0f;
-    if (tp < 1.0f) {
-        const u64 need = (u64)(((u128)max(1u, fixed24(tp)) * z + (kOne - 1u)) >> 24);
-        auto ok = [&](u64 s) { return (s & kMass) >= need; };
-        // after top-k within the weights above the k-th, which are all kept, if they suffice
-        if (ties == 0 || ok(shi)) {
-            if (ties) slo = shi;
-            shi = 0;
-            lo = bisect(row, w, ties ? lo + 1u : 1u, kOne + 1u, slo, shi, ok);
-        }
-    }
-    if (a.min_p) lo = max(lo, fixed24(a.min_p[r]));
-
     // The first token, in order, at which the running sum of the values that
     // f(sum, i, token, t) adds exceeds target(total); the values may carry the
     // tag. to_all: the index goes to every thread.
@@ -434,82 +394,157 @@ __global__ void __launch_bounds__(NT, NT >= 512 ? 1 : 512 / NT) sample_rows_kern
         return 0u;
     };
 
-    if (kth && lo == kth) {
-        // top-k keeps `room` of the `ties` weights equal to kth: the largest
-        // logits, equal ones in index order (different logits can share a weight,
-        // far below the maximum thousands of them)
-        constexpr uint32_t kHalf = 0x80000000u, kKept = 1u << 29;
-        const uint32_t tie = kth + kTag;
-        uint32_t top, bot;
-        auto range = [&]() {   // of the ties' keys
-            uint32_t hi = 0, lo_c = 0;
+    int k = a.top_k ? a.top_k[r] : 0;
+    uint32_t lo;   // kept: the weights >= lo
+    // Once, and once more without top-k where its cut lies among weights that are not
+    // ordered as their logits are (kUnorderedMin)
+    for (;;) {
+        // x / T rounded to nearest from one reciprocal (Markstein: with r the
+        // rounded 1 / T, q = x r corrected by r (x - q T) is the rounded quotient
+        // unless T's fraction is all ones), where neither it nor a quotient that
+        // gives a weight leaves the normal range; quotients beyond -17 give 0
+        const uint32_t tb = __float_as_uint(T);
+        if (T > 1e-20f && T < 1e20f && (tb & 0x7fffffu) != 0x7fffffu) {
+            const float rt = __frcp_rn(T), low = -18.0f * T;
 #pragma unroll
-            for (int j = 0; j < J; j++)
+            for (int i = 0; i < kTok; i++) {
+                const float x = __fsub_rn(__uint_as_float(w[i]), mx);
+                const float xc = fmaxf(x, low);   // its weight is 0 too, and its quotient in range
+                const float q0 = __fmul_rn(xc, rt);
+                w[i] = sample_weight(__fmaf_rn(__fmaf_rn(-q0, T, xc), rt, q0)) + kTag;
+            }
+        } else {
 #pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (w[j * VEC + e] == tie) {
-                        const uint32_t s = sortable(logit<DT>(l, token(j, e)));
-                        hi = max(hi, s);
-                        lo_c = max(lo_c, ~s);
-                    }
-            top = row.max32(hi);
-            bot = ~row.max32(lo_c);
-        };
-        range();
-        u64 left = ties, need = room;
-        if (top - bot >= kHalf) {   // both signs, a vast temperature: the one that the cut lies in
-            uint32_t c = 0;
-#pragma unroll
-            for (int j = 0; j < J; j++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (w[j * VEC + e] == tie) c += sortable(logit<DT>(l, token(j, e))) >= kHalf;
-            const u64 pos = row.sum(0, c);
-            const bool up = pos >= need;
-#pragma unroll
-            for (int j = 0; j < J; j++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (w[j * VEC + e] == tie && (sortable(logit<DT>(l, token(j, e))) >= kHalf) != up)
-                        w[j * VEC + e] = up ? kTag : tie | kKept;   // dropped, or kept without more ado
-            left = up ? pos : left - pos;
-            need = up ? need : need - pos;
-            range();
+            for (int i = 0; i < kTok; i++) w[i] = sample_weight(__fdiv_rn(__fsub_rn(__uint_as_float(w[i]), mx), T)) + kTag;
         }
-        if (need < left) {
-            // the ties as their keys less the smallest, below 2^31, marked by the top bit
-#pragma unroll
-            for (int j = 0; j < J; j++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (w[j * VEC + e] == tie)
-                        w[j * VEC + e] = kHalf + (sortable(logit<DT>(l, token(j, e))) - bot);
-            // cut: as many keys at or above it as are needed, or the largest with at least as many
-            uint32_t cut = kHalf, end = kHalf + (top - bot) + 1u;
-            u64 at_cut = left, at_end = 0;
-            while (end - cut > 1u && at_cut != need) {
-                const uint32_t mid = cut + (end - cut) / 2u;
+        const u64 all = at_least(row, w, 1u);
+        u64 slo = all, shi = 0;
+        lo = 1u;
+        u64 z = all & kMass;
+        u64 ties = 0, room = 0;    // weights equal to lo, and how many of them top-k keeps
+        bool apart = false;        // ties are those of lo - 1 and lo + 1, too
+        if (k > 0 && (u64)k < (all >> kMassBits)) {
+            lo = bisect(row, w, 1u, kOne + 1u, slo, shi, [&](u64 s) { return (s >> kMassBits) >= (u64)k; });
+            ties = (slo - shi) >> kMassBits;
+            room = (u64)k - (shi >> kMassBits);
+            z = (shi & kMass) + room * lo;
+            if (lo >= kUnorderedMin && lo <= kUnorderedMax) {
+                const uint32_t from = lo - 1u + kTag;
                 uint32_t c = 0;
 #pragma unroll
-                for (int i = 0; i < kTok; i++) c += w[i] >= mid;
+                for (int i = 0; i < kTok; i++) c += w[i] - from <= 2u;
                 const u64 n = row.sum(0, c);
-                if (n >= need) { cut = mid; at_cut = n; } else { end = mid; at_end = n; }
-            }
-            uint32_t last = 0xffffffffu;   // of the tokens at the cut, the last one kept
-            if (at_cut != need)
-                last = locate(cut, [&](uint32_t& sum, int i, int, uint32_t t) { sum += w[i] == t; },
-                              [&](u64) { return need - at_end - 1; }, true);
-#pragma unroll
-            for (int j = 0; j < J; j++)
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const uint32_t x = w[j * VEC + e];
-                    if (x >= kHalf)
-                        w[j * VEC + e] = x > cut || (x == cut && (uint32_t)token(j, e) <= last) ? tie : kTag;
+                apart = n != ties;
+                if (apart) {
+                    room = (u64)k - (at_least(row, w, lo + 2u) >> kMassBits);
+                    ties = n;
                 }
+            }
         }
+        const uint32_t kth = ties > room ? lo : 0u;   // the weight of which only some are kept
+        const float tp = a.top_p ? a.top_p[r] : 1.0f;
+        if (tp < 1.0f && !apart) {
+            const u64 need = (u64)(((u128)max(1u, fixed24(tp)) * z + (kOne - 1u)) >> 24);
+            auto ok = [&](u64 s) { return (s & kMass) >= need; };
+            // after top-k within the weights above the k-th, which are all kept, if they suffice
+            if (ties == 0 || ok(shi)) {
+                if (ties) slo = shi;
+                shi = 0;
+                lo = bisect(row, w, ties ? lo + 1u : 1u, kOne + 1u, slo, shi, ok);
+            }
+        }
+        if (a.min_p && !apart) lo = max(lo, fixed24(a.min_p[r]));
+
+        if (apart || (kth && lo == kth)) {
+            // top-k keeps `room` of the `ties` weights equal to lo (or next to it): the
+            // largest logits, equal ones in index order (different logits can share a
+            // weight, far below the maximum thousands of them)
+            constexpr uint32_t kHalf = 0x80000000u, kKept = 1u << 29;
+            const uint32_t tie = lo + kTag, from = tie - (apart ? 1u : 0u), span = apart ? 2u : 0u;
+            asm volatile("" : "+r"(first));   // nothing of the 64 addresses is kept from before
+            uint32_t top, bot;
+            auto range = [&]() {   // of the ties' keys
+                uint32_t hi = 0, lo_c = 0;
 #pragma unroll
-        for (int i = 0; i < kTok; i++) w[i] &= ~kKept;
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        if (w[j * VEC + e] - from <= span) {
+                            const uint32_t s = sortable(logit<DT>(l, token(j, e)));
+                            hi = max(hi, s);
+                            lo_c = max(lo_c, ~s);
+                        }
+                top = row.max32(hi);
+                bot = ~row.max32(lo_c);
+            };
+            range();
+            u64 left = ties, need = room;
+            if (top - bot >= kHalf) {   // both signs, a vast temperature: the one that the cut lies in
+                uint32_t c = 0;
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        if (w[j * VEC + e] - from <= span) c += sortable(logit<DT>(l, token(j, e))) >= kHalf;
+                const u64 pos = row.sum(0, c);
+                const bool up = pos >= need;
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        if (w[j * VEC + e] - from <= span && (sortable(logit<DT>(l, token(j, e))) >= kHalf) != up)
+                            w[j * VEC + e] = up ? kTag : w[j * VEC + e] | kKept;   // dropped, or kept without more ado
+                left = up ? pos : left - pos;
+                need = up ? need : need - pos;
+                range();
+            }
+            if (need < left) {
+                // the ties as their keys less the smallest, below 2^31, marked by the top bit
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        if (w[j * VEC + e] - from <= span)
+                            w[j * VEC + e] = kHalf + (sortable(logit<DT>(l, token(j, e))) - bot);
+                // cut: as many keys at or above it as are needed, or the largest with at least as many
+                uint32_t cut = kHalf, end = kHalf + (top - bot) + 1u;
+                u64 at_cut = left, at_end = 0;
+                while (end - cut > 1u && at_cut != need) {
+                    const uint32_t mid = cut + (end - cut) / 2u;
+                    uint32_t c = 0;
+#pragma unroll
+                    for (int i = 0; i < kTok; i++) c += w[i] >= mid;
+                    const u64 n = row.sum(0, c);
+                    if (n >= need) { cut = mid; at_cut = n; } else { end = mid; at_end = n; }
+                }
+                uint32_t last = 0xffffffffu;   // of the tokens at the cut, the last one kept
+                if (at_cut != need)
+                    last = locate(cut, [&](uint32_t& sum, int i, int, uint32_t t) { sum += w[i] == t; },
+                                  [&](u64) { return need - at_end - 1; }, true);
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        const uint32_t x = w[j * VEC + e];
+                        if (x >= kHalf)
+                            w[j * VEC + e] = x > cut || (x == cut && (uint32_t)token(j, e) <= last) ? tie : kTag;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < kTok; i++) w[i] &= ~kKept;
+            if (apart) {   // the logits that top-k keeps; the other rules on them alone
+                asm volatile("" : "+r"(first));
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        w[j * VEC + e] =
+                            __float_as_uint(w[j * VEC + e] >= from ? logit<DT>(l, token(j, e)) : -INFINITY);
+                k = 0;
+                continue;
+            }
+        }
+        break;
     }
     const uint32_t U = min(fixed24(a.u[r]), kOne - 1u);
     locate(lo + kTag, [&](uint32_t& sum, int i, int, uint32_t t) { add_if_ge(sum, w[i], t, row.one); },

@@ -111,6 +111,63 @@ def test_many_rows(gpu, orc, dtype, V):
           rng.uniform(0, 0.05, R))
 
 
+def test_order_of_the_weights(tmp_path):
+    """What the kernel's top-k relies on: weights are ordered as their logits but
+    for differences of one between the two named constants (every float gone
+    through in C)."""
+    import os
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("needs gcc")
+    here = os.path.dirname(os.path.abspath(__file__))
+    exe = tmp_path / "sample_weight_check"
+    subprocess.run(["gcc", "-O3", "-march=native", "-ffp-contract=off", "-o", str(exe),
+                    os.path.join(here, "sample_weight_check.c"), "-lm"], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600, check=True)
+    assert r.stdout == f"below 1 floats 2878 weights 13066122 to 16518617 largest {ONE}\n"
+    src = open(os.path.join(os.path.dirname(flb200.LIB_PATH), "csrc", "sample_rows.cu")).read()
+    assert "kUnorderedMin = 13066122u, kUnorderedMax = 16518617u" in src
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 5000, 30000, 100000])
+def test_top_k_is_by_logits(gpu, orc, V):
+    """A pair of neighbouring logits of which the larger has the smaller weight,
+    at the cut of top-k: alone (the other logits far below), and in a row so hot
+    that the cut lies in a crowd of such weights."""
+    import torch
+    a, b = np.float32(-0.224945396), np.float32(-0.224945411)
+    E, _ = orc.sample_weights(np.array([0, a, b], np.float32), 1.0, 1.0)
+    assert a > b and E[1] < E[2]
+    rng = np.random.default_rng(V)
+    l = np.full((6, V), -9.0, np.float32)
+    for r in range(6):
+        l[r, rng.permutation(V)[:3]] = np.roll([0, a, b], r)
+    d = torch.tensor(l, device="cuda")
+    for u in (0.0, 0.3, 0.55, 0.9, 0.9999):
+        for k in (1, 2, 3):
+            for p in (None, [0.7] * 6, [0.99] * 6):
+                check(gpu, orc, d, [u] * 6, None, [k] * 6, p, None)
+    for dtype in ("float32", "bfloat16"):
+        hot = make(rng, 6, V, dtype, 8.0)
+        for T in (40.0, 150.0, 400.0):
+            for k in (2, max(2, V // 3), V - 1):
+                check(gpu, orc, hot, rng.random(6), [T] * 6, [k] * 6, None, None)
+                check(gpu, orc, hot, rng.random(6), [T] * 6, [k] * 6, [0.8] * 6, [0.0, 0.9, 0.95, 0.0, 0.5, 1.0])
+    # the cut within a crowd of one unordered pair's floats
+    x = np.where(rng.random((6, V)) < 0.5, a, b).astype(np.float32)
+    x[:, 0] = 0.0
+    d = torch.tensor(x, device="cuda")
+    for k in sorted({2, V // 2 + 1, V - 1}):
+        check(gpu, orc, d, rng.random(6), None, [k] * 6, None, None)
+    # weights next to each other of logits of both signs, far below the largest
+    far = make(rng, 6, V, "float32", 3.0)
+    far[:, 1] = 1e7
+    for k in sorted({2, V // 2 + 1, V - 1}):
+        check(gpu, orc, far, rng.random(6), [5e7] * 6, [k] * 6, None, None)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("R,V", [(160, 8000), (160, 20000), (8, 20000), (24, 60000), (12, 200000)])
 def test_top_p_right_behind_a_small_top_k(gpu, orc, R, V):
