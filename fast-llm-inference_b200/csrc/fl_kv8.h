@@ -94,7 +94,12 @@ struct Kv8Tiles {
     float* part;
     float2* part_ml;
     int* part_cnt;
+    // the prefill kernel's bounded waits; fail_at > 0: the issuing thread of CTA
+    // fail_cta stops before its fail_at-th group of products, as if a wait had run out
+    long long wait_clocks;
+    int fail_cta, fail_at;
 };
+constexpr long long kKv8WaitClocks = 4000000000ll;   // about 2 s
 cudaError_t launch_kv8_attention(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s);
 cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int ctas, cudaStream_t s);
 // CTAs of the attention kernel that one SM holds (for the plan's split).

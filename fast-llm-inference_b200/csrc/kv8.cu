@@ -802,8 +802,16 @@ FL_API int fl_kv8_gather(fl_kv8_t* h, int layer, void* k, void* v, int keys, voi
     return FL_OK;
 }
 
-FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo,
-                            float scale, const uint8_t* mask, int ldm, void* stream) {
+namespace {
+
+// How a call's bounded waits behave: their limit, and a CTA that gives up (fl_kv8.h).
+struct Waits {
+    long long clocks = kKv8WaitClocks;
+    int fail_cta = 0, fail_at = 0;
+};
+
+int attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo, float scale,
+              const uint8_t* mask, int ldm, const Waits& wait, void* stream) {
     FL_CHECK(check_layer(h, layer, "kv8_attention"));
     if (rows < 0) return set_error(FL_E_INVAL, "kv8_attention: rows is negative");
     if (rows == 0) return FL_OK;
@@ -841,8 +849,23 @@ FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, in
     p.ldm = ldm;
     Kv8Tiles tl[2];
     for (int i = 0; i < 2; i++)
-        tl[i] = Kv8Tiles{i, h->t.tile_start[i], h->t.work_start[i], h->part[i], h->part_ml[i], h->part_cnt[i]};
+        tl[i] = Kv8Tiles{i, h->t.tile_start[i], h->t.work_start[i], h->part[i], h->part_ml[i], h->part_cnt[i],
+                         wait.clocks, wait.fail_cta, wait.fail_at};
     FL_CHECK_CUDA(launch_kv8_attention(p, tl[0], h->parts[0], s));
     if ((long long)h->max_new * h->group >= long_min(h)) FL_CHECK_CUDA(launch_kv8_prefill(p, tl[1], h->parts[1], s));
     return FL_OK;
+}
+
+}  // namespace
+
+FL_API int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo,
+                            float scale, const uint8_t* mask, int ldm, void* stream) {
+    return attention(h, layer, q, out, rows, ldq, ldo, scale, mask, ldm, Waits{}, stream);
+}
+
+FL_API int fl_kv8_wait_timeout_check(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo,
+                                     float scale, int cta, int at, void* stream) {
+    if (cta < 0 || at < 1) return set_error(FL_E_INVAL, "kv8_wait_timeout_check: cta or at is out of range");
+    // every other wait of that CTA runs out, too: a tenth of a second each
+    return attention(h, layer, q, out, rows, ldq, ldo, scale, nullptr, 0, Waits{200000000ll, cta, at}, stream);
 }

@@ -29,8 +29,8 @@
 // Prompt chunks of 0.8 to 2 k rows behind 0 to 6 k keys (32 / 8 heads of 128, 0.34
 // TFLOP) take 0.85 ms, 0.4 PFLOP/s; the row kernel takes 2.47 ms.
 //
-// Waits are bounded (4e9 clocks, about 2 s); on expiry the CTA raises an error word,
-// stops, waits (bounded) for its own products, frees TMEM and exits.
+// Waits are bounded (kKv8WaitClocks, about 2 s); on expiry the CTA raises an error word,
+// stops, waits (bounded) for all products that it issued, frees TMEM and exits.
 #include <math.h>
 
 #include <algorithm>
@@ -49,7 +49,6 @@ __device__ int g_kv8_error = 0;
 constexpr int kRows = 128;               // query rows of a tile
 constexpr int kPair = kKv8Long;          // of a CTA's two tiles
 constexpr int kThreads = 13 * 32;
-constexpr long long kWaitClocks = 4000000000ll;   // about 2 s
 constexpr float kVUp = 32.0f;            // V enters as 2^5 code / largest scale: 1152 2^5, the offset, is a half
 
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -68,11 +67,11 @@ __device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t par) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t par) {
+__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t par, long long limit) {
     if (mb_try(b, par)) return true;
     const long long t0 = clock64();
     while (!mb_try(b, par))
-        if (clock64() - t0 > kWaitClocks) {
+        if (clock64() - t0 > limit) {
             atomicOr(&g_kv8_error, 1);
             return false;
         }
@@ -81,8 +80,8 @@ __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t par) {
 // By a whole warp: every lane polls, so that the warp stays together (one lane
 // polling for the others left it in two pieces that ran the code after it in turn:
 // 3 times the time per page).
-__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t par) {
-    const bool ok = mb_wait(b, par);
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t par, long long limit) {
+    const bool ok = mb_wait(b, par, limit);
     return __all_sync(0xffffffffu, ok);
 }
 
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int NC = HD / 32;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) TileBars bars[2];
-    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
     __shared__ uint32_t tmem_s;
     __shared__ int bad_s;
     __shared__ Kv8Joins joins;
@@ -263,6 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mb_init(&v_full[i], 4);
             mb_init(&v_empty[i], 1);
         }
+        mb_init(&drained, 1);
         bad_s = joins.n = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float4 ks4 = next.k;
                 const float vs = vscale_max(next.v, k0 + j * kPageSize, ctx + nb);
                 next.load(p, bt, h, j + 1, n);
-                if (!warp_wait(&bar.s_full[J & 1], (J >> 1) & 1)) { ok = false; break; }
+                if (!warp_wait(&bar.s_full[J & 1], (J >> 1) & 1, tl.wait_clocks)) { ok = false; break; }
                 tc_after();
                 const uint32_t sb = tq + (J & 1) * 64;
                 const float f[4] = {ks4.x * unshift, ks4.y * unshift, ks4.z * unshift, ks4.w * unshift};
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     l *= al;
                     const float g = al * (vref * pow2_inv(vnew));
                     // O: the products of the page before have to be done
-                    if (!warp_wait(&bar.pv_done, (J - 1) & 1)) { ok = false; break; }
+                    if (!warp_wait(&bar.pv_done, (J - 1) & 1, tl.wait_clocks)) { ok = false; break; }
                     tc_after();
 #pragma unroll 1
                     for (int c = 0; c < 2 * NC; c++) {
@@ -441,15 +441,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 // the page before is done with, usually long ago: no thread falls two phases
                 // of pv_done behind, which its parity could not tell apart
-                if (j > 0 && !warp_wait(&bar.pv_done, (J - 1) & 1)) { ok = false; break; }
+                if (j > 0 && !warp_wait(&bar.pv_done, (J - 1) & 1, tl.wait_clocks)) { ok = false; break; }
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mb_arrive(&bar.p_full[J & 1]);
             }
             // the row's output: normalised, to its place or to the part's slot
-            if (ok && n > 0) ok = warp_wait(&bar.pv_done, (jb + n - 1) & 1);
+            if (ok && n > 0) ok = warp_wait(&bar.pv_done, (jb + n - 1) & 1, tl.wait_clocks);
             if (!ok) {
+                tmem_wait_st();   // P or O may still be on its way to TMEM
+                tc_before();
                 if (lane == 0) atomicOr(&bad_s, 1);
             } else {
                 tc_after();
@@ -550,23 +552,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float4 vs4 = next.v;
                 const int after = next.page;   // of page j + 1
                 next.load(p, bt, h, j + 1, n);
-                if (J > 1 && !warp_wait(&k_empty[st], par)) { ok = false; break; }
+                if (J > 1 && !warp_wait(&k_empty[st], par, tl.wait_clocks)) { ok = false; break; }
                 write_k(st);
                 if (j + 1 < n) load_k(after);
-                if (J > 1 && !warp_wait(&v_empty[st], par)) { ok = false; break; }
+                if (J > 1 && !warp_wait(&v_empty[st], par, tl.wait_clocks)) { ok = false; break; }
                 write_v(st, j, vs4);
                 if (j + 1 < n) load_v();
             }
             if (!ok && lane == 0) atomicOr(&bad_s, 1);
         } else if (warp == 12 && lane == 0) {
             // ------------------------------------------------------ products
+            int fail = (int)blockIdx.x == tl.fail_cta ? tl.fail_at : 0;
             auto scores = [&](int tile, int j) -> bool {   // S of page j of a tile
                 const uint32_t J = J0 + j, T = (tile ? jt1 : jt0) + j;
                 // over P of the tile's page before last: its product has to be done (the
                 // items before are; their phase could be mistaken for a later one's)
-                if (j > 1 && !mb_wait(&bars[tile].pv_done, (T - 2) & 1)) return false;
-                if (j == 0 && !mb_wait(&bars[tile].q_full, (tile ? items1 : items0) & 1)) return false;
-                if (!mb_wait(&k_full[J & 1], (J >> 1) & 1)) return false;
+                if (j > 1 && !mb_wait(&bars[tile].pv_done, (T - 2) & 1, tl.wait_clocks)) return false;
+                if (j == 0 && !mb_wait(&bars[tile].q_full, (tile ? items1 : items0) & 1, tl.wait_clocks)) return false;
+                if (!mb_wait(&k_full[J & 1], (J >> 1) & 1, tl.wait_clocks)) return false;
+                if (fail && --fail == 0) return false;
                 tc_after();
 #pragma unroll
                 for (int q = 0; q < L::kParts; q++)
@@ -584,7 +588,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             auto output = [&](int tile, int j) -> bool {   // O (+)= P V of page j of a tile
                 const uint32_t J = J0 + j, T = (tile ? jt1 : jt0) + j;
-                if (!mb_wait(&v_full[J & 1], (J >> 1) & 1) || !mb_wait(&bars[tile].p_full[T & 1], (T >> 1) & 1)) return false;
+                if (!mb_wait(&v_full[J & 1], (J >> 1) & 1, tl.wait_clocks) ||
+                    !mb_wait(&bars[tile].p_full[T & 1], (T >> 1) & 1, tl.wait_clocks))
+                    return false;
+                if (fail && --fail == 0) return false;
                 tc_after();
 #pragma unroll
                 for (int q = 0; q < L::kParts; q++)
@@ -597,23 +604,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return true;
             };
             bool ok = true;
-            int nqk = 0, npv = 0;   // pages whose products are issued, of all tiles
             if (n > 0)
                 ok = scores(0, 0) && (nt == 1 || scores(1, 0));
-            nqk = ok && n > 0;
             for (int j = 0; j < n && ok; j++) {
                 ok = (j + 1 >= n || scores(0, j + 1)) && output(0, j);
                 if (nt > 1) ok = ok && (j + 1 >= n || scores(1, j + 1)) && output(1, j);
-                if (ok) {
-                    nqk = min(j + 2, n);
-                    npv = j + 1;
-                }
             }
-            if (!ok) {   // the products under way read this CTA's memory: wait for them, too
-                if (nqk > 0) (void)mb_wait(&k_empty[(J0 + nqk - 1) & 1], ((J0 + nqk - 1) >> 1) & 1);
-                if (npv > 0) (void)mb_wait(&v_empty[(J0 + npv - 1) & 1], ((J0 + npv - 1) >> 1) & 1);
-                atomicOr(&bad_s, 1);
-            }
+            if (!ok) atomicOr(&bad_s, 1);
         }
         __syncthreads();
         if (bad_s) break;
@@ -628,6 +625,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncthreads();
     }
     __syncthreads();
+    if (bad_s) {
+        // products under way read this CTA's memory and write its TMEM, whichever wait
+        // ran out: all that were issued signal `drained`
+        if (warp == 12 && lane == 0) {
+            atomicOr(&g_kv8_error, 1);
+            umma_commit(&drained);
+            (void)mb_wait(&drained, 0, tl.wait_clocks);
+        }
+        __syncthreads();
+    }
     if (warp == 12) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));

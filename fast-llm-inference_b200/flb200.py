@@ -139,6 +139,7 @@ _SIGS = {
     "fl_kv8_plan": (I, [VP, VP, VP, I, I, VP]),
     "fl_kv8_append": (I, [VP, I, VP, VP, I, SZ, SZ, VP]),
     "fl_kv8_attention": (I, [VP, I, VP, VP, I, SZ, SZ, F, VP, I, VP]),
+    "fl_kv8_wait_timeout_check": (I, [VP, I, VP, VP, I, SZ, SZ, F, I, I, VP]),
     "fl_kv8_gather": (I, [VP, I, VP, VP, I, VP]),
     "fl_cuda_sample": (I, [VP, I, SZ, I, I, VP, VP, VP, VP, VP, VP, VP]),
     "fl_synth_q4_0_i8": (I, [U64, U32, I, I, F, VP, VP]),

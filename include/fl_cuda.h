@@ -166,7 +166,9 @@ int fl_cuda_block_dots_i8_noalloc(const float* A, const dequantized_tensor_t* B,
  * that the host knew: a captured attention holds for plans whose max_new is no
  * larger than at its capture, a captured append or gather for no more sequences.
  * The attention's waits on the device are bounded; one that gave up leaves
- * outputs unwritten, and the next fl_cuda_sync returns FL_E_TIMEOUT. `stream` NULL is the library's stream; pass cudaStreamLegacy
+ * outputs unwritten, and the first fl_cuda_sync after that call's end returns
+ * FL_E_TIMEOUT (it waits for the library's stream: wait for a stream of your own
+ * before it). `stream` NULL is the library's stream; pass cudaStreamLegacy
  * ((void*)1) for CUDA's default stream. FL_E_STATE when the current device is
  * not the handle's, or not that of an array; FL_E_INVAL for host memory. */
 #define FL_F32  0
@@ -241,6 +243,14 @@ int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, int rows
  * summed in 32 bits; f32 queries and their probabilities keep 22 bits. */
 int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo, float scale,
                      const uint8_t* mask, int ldm, void* stream);
+
+/* Failure detection: a causal fl_kv8_attention in which CTA `cta` of the kernel
+ * for many rows gives up before its `at`-th group of products (from 1; none if it
+ * has fewer), as if a wait had run out. Its other waits then run out, after a tenth
+ * of a second; it raises the error word and returns. The following fl_cuda_sync()
+ * returns FL_E_TIMEOUT and clears the word, and the device stays usable. */
+int fl_kv8_wait_timeout_check(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo,
+                              float scale, int cta, int at, void* stream);
 
 /* The values that the codes of every planned sequence with new rows stand for,
  * its cached and new positions in order, sequences one after another (kv_start):

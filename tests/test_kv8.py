@@ -689,3 +689,47 @@ def test_first_launches_of_a_process(gpu):
     code = f"import sys; sys.path[:0] = {[here, os.path.dirname(flb200.LIB_PATH)]!r}; import test_kv8; test_kv8.cold_attention()"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ------------------------------------------------------- waits that run out
+def long_rows(gpu, rng, dtype="bfloat16", ctx=3000, new=300):
+    """One sequence whose tiles several CTAs of the kernel for many rows share."""
+    p = Pair(gpu, heads=2, kv_heads=1, hd=64, dtype=dtype, pages=80, max_seqs=1, max_rows=4000, max_ctx=4000)
+    p.plan([0], [ctx], check=False)
+    p.append(p.rows(rng, 1), p.rows(rng, 1))
+    p.plan([ctx], [new], check=False)
+    p.append(p.rows(rng, 1), p.rows(rng, 1))
+    return p, p.rows(rng, 2)
+
+
+def give_up(gpu, p, q, cta, at):
+    out = torch.full_like(q, 9.0)
+    rc = gpu.fl_kv8_wait_timeout_check(p.c.h, 0, q.data_ptr(), out.data_ptr(), q.shape[0], q.stride(0), q.stride(0),
+                                       p.hd ** -0.5, cta, at, None)
+    assert rc == 0, gpu.err()
+    return out
+
+
+def test_timeout_check_refuses(lib):
+    for cta, at in ((-1, 1), (0, 0)):
+        assert lib.fl_kv8_wait_timeout_check(None, 0, 64, 64, 1, 64, 64, 1.0, cta, at, None) == -1
+        assert "out of range" in lib.err()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_wait_that_runs_out_is_reported(gpu, dtype):
+    """A CTA that stops at any of its groups of products (before the first, between
+    the two tiles, with products of one tile under way) ends, reports, and
+    leaves the device usable."""
+    rng = np.random.default_rng(13)
+    other, oq = long_rows(gpu, rng, dtype)
+    for at in range(1, 10):
+        p, q = long_rows(gpu, rng, dtype)
+        torch.cuda.synchronize()
+        give_up(gpu, p, q, at % 3, at)
+        assert gpu.fl_cuda_sync() == -5, at
+        assert gpu.fl_cuda_sync() == 0
+        other.check_attention(oq)
+        torch.cuda.synchronize()
+    assert gpu.fl_cuda_sync() == 0
