@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ __align__(8) TileBars bars[2];
     __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
     __shared__ uint32_t tmem_s;
-    __shared__ int bad_s;
+    __shared__ int bad_s, fail_s;   // fail_s: groups of products before the CTA gives up, 0: it does not
     __shared__ Kv8Joins joins;
     __shared__ Kv8Item it;
     const uint32_t smem = (saddr(smem_raw) + 1023u) & ~1023u;
@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mb_init(&drained, 1);
         bad_s = joins.n = 0;
+        fail_s = (int)blockIdx.x == tl.fail_cta ? tl.fail_at : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -562,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok && lane == 0) atomicOr(&bad_s, 1);
         } else if (warp == 12 && lane == 0) {
             // ------------------------------------------------------ products
-            int fail = (int)blockIdx.x == tl.fail_cta ? tl.fail_at : 0;
+            int fail = fail_s;
             auto scores = [&](int tile, int j) -> bool {   // S of page j of a tile
                 const uint32_t J = J0 + j, T = (tile ? jt1 : jt0) + j;
                 // over P of the tile's page before last: its product has to be done (the
@@ -610,6 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = (j + 1 >= n || scores(0, j + 1)) && output(0, j);
                 if (nt > 1) ok = ok && (j + 1 >= n || scores(1, j + 1)) && output(1, j);
             }
+            fail_s = fail;
             if (!ok) atomicOr(&bad_s, 1);
         }
         __syncthreads();
