@@ -145,14 +145,21 @@ struct Kv8Joins {
     int n;
     Kv8Item item[2];
 };
+// A range arrives at its tile's count: the ranges so far, and above them those that
+// were given up. The last one clears the count, for the launches that follow; true
+// for it if all ranges have their results.
+constexpr int kGivenUp = 1 << 16;   // above any number of ranges
+__device__ __forceinline__ bool arrive_last(const Kv8Tiles& tl, const Kv8Item& it, int given_up) {
+    const int n = atomicAdd(tl.part_cnt + it.part, 1 + given_up) + given_up;
+    if ((n & (kGivenUp - 1)) != it.splits - 1) return false;
+    tl.part_cnt[it.part] = 0;
+    return n < kGivenUp;
+}
 // After a range's results are written (whole block).
 __device__ __forceinline__ void range_done(const Kv8Tiles& tl, const Kv8Item& it, Kv8Joins& joins) {
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0 && atomicAdd(tl.part_cnt + it.part, 1) == it.splits - 1) {
-        tl.part_cnt[it.part] = 0;
-        joins.item[joins.n++] = it;
-    }
+    if (threadIdx.x == 0 && arrive_last(tl, it, 0)) joins.item[joins.n++] = it;
 }
 
 // Rows 0 .. np - 1 of a tile joined from its parts' results, in the parts' order,

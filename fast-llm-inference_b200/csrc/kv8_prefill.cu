@@ -635,6 +635,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             umma_commit(&drained);
             (void)mb_wait(&drained, 0, tl.wait_clocks);
         }
+        // the tiles that other CTAs share with this one are not joined, by none of them,
+        // and their counts start from zero again
+        if (warp == 0)
+            while (it.pages) {
+                if (lane == 0 && it.splits > 1) (void)arrive_last(tl, it, kGivenUp);
+                const long long x = it.next;
+                __syncwarp();
+                next_item(p, tl, x, lane, it);
+                __syncwarp();
+            }
         __syncthreads();
     }
     if (warp == 12) {

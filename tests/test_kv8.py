@@ -733,3 +733,24 @@ def test_a_wait_that_runs_out_is_reported(gpu, dtype):
         other.check_attention(oq)
         torch.cuda.synchronize()
     assert gpu.fl_cuda_sync() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_cache_is_usable_after_a_wait_that_ran_out(gpu, dtype):
+    """Tiles that several CTAs share, of which one gave up: they are left unwritten,
+    whoever arrives last; the next call on the cache joins them as ever."""
+    rng = np.random.default_rng(14)
+    p, q = long_rows(gpu, rng, dtype)
+    right = p.check_attention(q)
+    for cta, at in ((0, 1), (3, 5), (7, 2), (8, 1), (11, 20), (25, 3), (17, 9)):
+        torch.cuda.synchronize()
+        out = give_up(gpu, p, q, cta, at)
+        assert gpu.fl_cuda_sync() == -5, cta
+        same = (out == right).flatten(1).all(1)
+        unwritten = (out == 9.0).flatten(1).all(1)
+        assert (same | unwritten).all() and unwritten.any(), cta
+        for _ in range(2):
+            q2 = p.rows(rng, 2)
+            p.check_attention(q2)
+        assert torch.equal(p.check_attention(q), right)
