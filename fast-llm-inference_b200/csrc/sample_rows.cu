@@ -617,8 +617,16 @@ FL_API int fl_cuda_sample(const void* logits, int dtype, size_t ld, int rows, in
     if (rows > 1 && ld < (size_t)V) return set_error(FL_E_INVAL, "sample: the row stride is below V");
     if ((uintptr_t)logits % (dtype == FL_F32 ? 4 : 2))
         return set_error(FL_E_INVAL, "sample: logits are not aligned to their type");
+    const struct {
+        const void* p;
+        const char* name;
+    } arrays[] = {{temperature, "sample: temperature"}, {top_k, "sample: top_k"}, {top_p, "sample: top_p"},
+                  {min_p, "sample: min_p"},             {u, "sample: u"},         {tokens, "sample: tokens"}};
+    for (const auto& x : arrays)
+        if ((uintptr_t)x.p % 4) return set_error(FL_E_INVAL, std::string(x.name) + " is not aligned to its type");
     FL_CHECK(check_device_ptr(logits, "sample: logits"));
-    FL_CHECK(check_device_ptr(tokens, "sample: tokens"));
+    for (const auto& x : arrays)
+        if (x.p) FL_CHECK(check_device_ptr(x.p, x.name));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
     const SampleArgs a = {logits, ld, V, 0, rows, 0, temperature, top_p, min_p, u, top_k, tokens};
     FL_CHECK_CUDA(dtype == FL_F32 ? sample_dt<FL_F32>(a, rows, s)

@@ -29,6 +29,15 @@ def test_refusals(lib):
     assert rc(V=262001, ld=262001) == -4
 
 
+def test_misaligned_arrays_are_refused(lib):
+    f = lib.fl_cuda_sample
+    ok = dict(logits=64, dtype=0, ld=8, rows=1, V=8, t=64, k=64, p=64, m=64, u=64, tok=64, s=None)
+    for name, arg in (("temperature", "t"), ("top_k", "k"), ("top_p", "p"), ("min_p", "m"), ("u", "u"), ("tokens", "tok")):
+        for at in (65, 66):
+            assert f(*dict(ok, **{arg: at}).values()) == -1
+            assert lib.err() == f"sample: {name} is not aligned to its type"
+
+
 def expect(orc, l, T, k, p, m, u):
     """The rule for one row of float32 logits."""
     l = np.where(np.isnan(l), -np.inf, np.minimum(l, np.finfo(np.float32).max)).astype(np.float32) + np.float32(0)
@@ -220,6 +229,21 @@ def test_host_memory_is_refused(gpu):
     assert f(flb200.ptr(host), 0, 100, 2, 100, None, None, None, None, l.data_ptr(), t.data_ptr(), None) == -1
     assert "not device memory" in gpu.err()
     assert f(l.data_ptr(), 0, 100, 2, 100, None, None, None, None, l.data_ptr(), flb200.ptr(host), None) == -1
+
+
+@pytest.mark.gpu
+def test_host_memory_of_any_array_is_refused(gpu):
+    import torch
+    l = torch.zeros((2, 100), device="cuda")
+    t = torch.zeros(2, dtype=torch.int32, device="cuda")
+    host = np.zeros(200, np.float32)
+    names = ("temperature", "top_k", "top_p", "min_p", "u", "tokens")
+    for i, name in enumerate(names):
+        arr = [l.data_ptr()] * 5 + [t.data_ptr()]
+        arr[i] = flb200.ptr(host)
+        assert gpu.fl_cuda_sample(l.data_ptr(), 0, 100, 2, 100, *arr, None) == -1
+        assert gpu.err() == f"sample: {name} is not device memory"
+    assert gpu.fl_cuda_sync() == 0
 
 
 @pytest.mark.gpu
