@@ -709,6 +709,8 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     if (!ctx_len || !new_len) return set_error(FL_E_INVAL, "kv8_plan: NULL lengths");
     if (nseq < 1 || nseq > h->c.max_seqs) return set_error(FL_E_INVAL, "kv8_plan: nseq must be 1 .. max_seqs");
     if (max_new < 1) return set_error(FL_E_INVAL, "kv8_plan: max_new must be at least 1");
+    if (((uintptr_t)ctx_len | (uintptr_t)new_len) % sizeof(int))
+        return set_error(FL_E_INVAL, "kv8_plan: lengths are not aligned to their type");
     FL_CHECK(check_device_ptr(ctx_len, "kv8_plan: ctx_len"));
     FL_CHECK(check_device_ptr(new_len, "kv8_plan: new_len"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
@@ -825,6 +827,7 @@ int attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t
     if (mask && ldm < h->max_new) return set_error(FL_E_INVAL, "kv8_attention: mask rows are shorter than max_new");
     FL_CHECK(check_device_ptr(q, "kv8_attention: q"));
     FL_CHECK(check_device_ptr(out, "kv8_attention: out"));
+    if (mask) FL_CHECK(check_device_ptr(mask, "kv8_attention: mask"));
     cudaStream_t s = stream ? (cudaStream_t)stream : device_stream();
     Kv8AttnParams p = {};
     p.k = h->k[layer];

@@ -754,3 +754,18 @@ def test_a_cache_is_usable_after_a_wait_that_ran_out(gpu, dtype):
             q2 = p.rows(rng, 2)
             p.check_attention(q2)
         assert torch.equal(p.check_attention(q), right)
+
+
+@pytest.mark.gpu
+def test_masks_in_host_memory_and_misaligned_lengths_are_refused(gpu):
+    p = Pair(gpu)
+    p.plan([0], [2])
+    q = torch.zeros((2, 4, 64), device="cuda")
+    host = np.ones((2, 2), np.uint8)
+    assert gpu.fl_kv8_attention(p.c.h, 0, q.data_ptr(), q.data_ptr(), 2, 256, 256, 1.0, flb200.ptr(host), 2, None) == -1
+    assert gpu.err() == "kv8_attention: mask is not device memory"
+    n = torch.zeros(8, dtype=torch.int32, device="cuda")
+    for a, b in ((1, 0), (0, 2)):
+        assert gpu.fl_kv8_plan(p.c.h, n.data_ptr() + a, n.data_ptr() + b, 1, 1, None) == -1
+        assert "not aligned" in gpu.err()
+    assert gpu.fl_cuda_sync() == 0
