@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                     for (int e = 0; e < 4; e++) {
                         const int j = pos0 + 4 * t4 + e - ctx;   // new row, negative: cached
                         bool see = j <= tok[r];
-                        if (p.mask && j >= 0) see = j < nb && live[r] && p.mask[(size_t)row[r] * p.ldm + j] != 0;
+                        if (p.mask && j >= 0) see = j < min(nb, p.ldm) && live[r] && p.mask[(size_t)row[r] * p.ldm + j] != 0;
                         if (!see) s[r][e] = -INFINITY;
                     }
             }

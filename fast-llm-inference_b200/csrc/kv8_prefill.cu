@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0 && n > 0) mb_arrive(&bar.q_full);
             const uint32_t tq = tmem + tile * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
             float m = -INFINITY, l = 0.0f, vref = 0.0f;
-            const int lim = p.mask ? ctx + nb : ctx + tok + 1;   // positions this row may see
+            const int lim = ctx + (p.mask ? min(nb, p.ldm) : tok + 1);   // positions this row may see
             // dead rows read some row of the mask, to no effect
             const uint8_t* mrow = p.mask + (size_t)(live ? row : min(row0, p.rows - 1)) * p.ldm;
             Scales next(p, bt, h, n);

@@ -237,7 +237,8 @@ int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, int rows
 /* out = softmax(scale * q K^T) V for every planned row and query head (rows
  * ldq / ldo elements apart), over its sequence's positions: the cached ones
  * and, of the new ones, those at or before the row's (mask NULL) or those that
- * mask[row * ldm + j] names for the sequence's j-th new row (ldm >= max_new).
+ * mask[row * ldm + j] names for the sequence's j-th new row (ldm >= max_new; new
+ * rows behind ldm, of a plan replayed from a graph, are not seen).
  * A row that sees nothing gives zeros. Rows behind the last planned one, and
  * behind `rows`, are left as they were. Products are taken with halves and
  * summed in 32 bits; f32 queries and their probabilities keep 22 bits. */

@@ -769,3 +769,45 @@ def test_masks_in_host_memory_and_misaligned_lengths_are_refused(gpu):
         assert gpu.fl_kv8_plan(p.c.h, n.data_ptr() + a, n.data_ptr() + b, 1, 1, None) == -1
         assert "not aligned" in gpu.err()
     assert gpu.fl_cuda_sync() == 0
+
+
+# ------------------------------------- plans replayed from a graph, calls made eagerly
+def replayed_plan(p, ctx, new, max_new, first, rng):
+    """A plan for up to max_new rows in a graph; behind its capture a small step is
+    planned by a call, then the graph is replayed with the lengths (ctx, new)."""
+    c, n = dev(ctx), dev(new)
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        p.c.plan(c, n, max_new, stream=s.cuda_stream)
+    p.plan([0] * len(ctx), ctx)
+    p.append(p.rows(rng, p.Hk), p.rows(rng, p.Hk))
+    p.plan(ctx, first)
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    p.m.plan(ctx, new, max_new)
+    p.check_tables()
+    p.append(p.rows(rng, p.Hk), p.rows(rng, p.Hk))
+    return g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[20, 3]])
+def test_masks_narrower_than_a_replayed_plan(gpu, new):
+    """New rows behind the mask's columns are not seen, nor read: the call's own
+    bound on new rows was that of the step planned by a call."""
+    rng = np.random.default_rng(15)
+    p = Pair(gpu, heads=2, kv_heads=2, hd=64)
+    g = replayed_plan(p, [40, 64], new, 200, [1, 1], rng)
+    T = sum(new)
+    mask = (rng.random((T, 2)) < 0.5).astype(np.uint8)
+    wide = np.zeros((T, max(new)), np.uint8)
+    wide[:, :2] = mask
+    q = p.rows(rng, 2)
+    got = torch.full_like(q, 9.0)
+    p.c.attention(0, q, got, 0.125, dev(mask, torch.uint8), stream=0)
+    want, parts = p.m.attention(q.double().cpu().numpy(), 0.125, wide)
+    assert (np.abs(got.double().cpu().numpy() - want) <= attention_bound("float32", want, parts, 64)).all()
+    del g
