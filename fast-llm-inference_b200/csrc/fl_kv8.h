@@ -62,6 +62,8 @@ struct fl_kv8 {
     int group = 1, tile_rows = 16;
     int parts[2] = {};          // CTAs of an attention launch, of either list's kernel
     int max_new = 0;            // bound of the last plan
+    int captured_max_new = 0;   // of all plans captured into graphs, which may be replayed at any time
+    unsigned long long plan_capture = 0;   // the capture that the last plan went into, 0: none
     int nseq = 0;
     std::vector<void*> bufs;
     std::vector<uint8_t*> k, v;       // [layers] codes

@@ -562,6 +562,17 @@ int check_layer(const fl_kv8* h, int layer, const char* what) {
     return FL_OK;
 }
 
+// The capture that a stream's calls go into, 0: none.
+unsigned long long capture_of(cudaStream_t s) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(s, &st, &id) != cudaSuccess) {   // the legacy stream while another one is captured
+        cudaGetLastError();
+        return 0;
+    }
+    return st == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 bool aligned(const void* p, size_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0; }
 
 template <typename T>
@@ -741,6 +752,8 @@ FL_API int fl_kv8_plan(fl_kv8_t* h, const int* ctx_len, const int* new_len, int 
     FL_CHECK_CUDA(cudaLaunchKernelEx(&cfg, small ? kv8_plan_kernel<256> : kv8_plan_kernel<1024>, a));
     h->nseq = nseq;
     h->max_new = a.max_new;
+    h->plan_capture = capture_of(s);
+    if (h->plan_capture) h->captured_max_new = std::max(h->captured_max_new, a.max_new);
     return FL_OK;
 }
 
@@ -855,7 +868,10 @@ int attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t
         tl[i] = Kv8Tiles{i, h->t.tile_start[i], h->t.work_start[i], h->part[i], h->part_ml[i], h->part_cnt[i],
                          wait.clocks, wait.fail_cta, wait.fail_at};
     FL_CHECK_CUDA(launch_kv8_attention(p, tl[0], h->parts[0], s));
-    if ((long long)h->max_new * h->group >= long_min(h)) FL_CHECK_CUDA(launch_kv8_prefill(p, tl[1], h->parts[1], s));
+    // The plan that this call will find may be a replayed one, unless both are in one capture
+    const bool own_plan = h->plan_capture && h->plan_capture == capture_of(s);
+    const long long max_new = own_plan ? h->max_new : std::max(h->max_new, h->captured_max_new);
+    if (max_new * h->group >= long_min(h)) FL_CHECK_CUDA(launch_kv8_prefill(p, tl[1], h->parts[1], s));
     return FL_OK;
 }
 

@@ -162,9 +162,11 @@ int fl_cuda_block_dots_i8_noalloc(const float* A, const dequantized_tensor_t* B,
  * append, attention and gather of a step are ordered by the caller's stream,
  * and captured graphs of one handle must not run at the same time. The calls
  * allocate nothing and can be captured; fl_kv8_plan re-reads the lengths at
- * every replay. The launches of a call are chosen by the bounds (rows, max_new)
- * that the host knew: a captured attention holds for plans whose max_new is no
- * larger than at its capture, a captured append or gather for no more sequences.
+ * every replay. The attention's launches are chosen by the largest max_new that
+ * the host knew: that of the last plan, or of a plan captured before. So a call, or
+ * a capture of the attention alone, serves the replays of every plan captured
+ * before it; where one capture takes in a plan and then the attention, that plan's
+ * max_new alone counts.
  * The attention's waits on the device are bounded; one that gave up leaves
  * outputs unwritten, and the first fl_cuda_sync after that call's end returns
  * FL_E_TIMEOUT (it waits for the library's stream: wait for a stream of your own

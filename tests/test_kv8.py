@@ -794,7 +794,7 @@ def replayed_plan(p, ctx, new, max_new, first, rng):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("new", [[20, 3]])
+@pytest.mark.parametrize("new", [[20, 3], [150, 3]])
 def test_masks_narrower_than_a_replayed_plan(gpu, new):
     """New rows behind the mask's columns are not seen, nor read: the call's own
     bound on new rows was that of the step planned by a call."""
@@ -810,4 +810,42 @@ def test_masks_narrower_than_a_replayed_plan(gpu, new):
     p.c.attention(0, q, got, 0.125, dev(mask, torch.uint8), stream=0)
     want, parts = p.m.attention(q.double().cpu().numpy(), 0.125, wide)
     assert (np.abs(got.double().cpu().numpy() - want) <= attention_bound("float32", want, parts, 64)).all()
+    del g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,new", [("float32", [130, 1]), ("bfloat16", [1, 150])])
+def test_attention_behind_a_replayed_plan(gpu, dtype, new):
+    """A prompt planned by a replay, after single tokens planned by a call: every row
+    is written, by an eager call and by a graph that holds the attention alone; a
+    graph of plan and attention for single tokens goes on beside them."""
+    rng = np.random.default_rng(16)
+    p = Pair(gpu, heads=4, kv_heads=2, hd=64, dtype=dtype)
+    ctx = [70, 9]
+    g = replayed_plan(p, ctx, new, 200, [1, 1], rng)
+    q = p.rows(rng, 4)
+    p.check_attention(q)
+    out = torch.full_like(q, 9.0)
+    s = torch.cuda.Stream()
+    alone, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    pos, one = dev([a + b for a, b in zip(ctx, new)]), dev([1, 1])
+    q1, k1 = q[:2].clone(), p.rows(rng, 2, 2)
+    out1 = torch.full_like(q1, 9.0)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(alone, stream=s):
+        p.c.attention(0, q, out, stream=s.cuda_stream)
+    with torch.cuda.graph(both, stream=s):
+        p.c.plan(pos, one, 1, stream=s.cuda_stream)
+        p.c.append(0, k1, k1, stream=s.cuda_stream)
+        p.c.attention(0, q1, out1, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    alone.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, p.check_attention(q))
+    both.replay()
+    torch.cuda.synchronize()
+    p.m.plan(pos.tolist(), [1, 1], 1)
+    p.m.append(k1.double().cpu().numpy(), k1.double().cpu().numpy())
+    want, parts = p.m.attention(q1.double().cpu().numpy(), 0.125)
+    assert (np.abs(out1.double().cpu().numpy() - want) <= attention_bound(dtype, want, parts, 64)).all()
     del g
