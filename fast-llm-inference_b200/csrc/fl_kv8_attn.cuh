@@ -15,6 +15,17 @@ constexpr float kTileCost = 3.0f, kJoinCost = 20.0f;   // in pages, see next_ite
 constexpr float kShift = 7.0f;   // probabilities enter as 2^7 p: 2^-21 of the largest is a normal half
 constexpr float kSlack = 8.0f;   // the reference follows the maximum once it lags by 2^8
 
+// The accumulators' scale is that of a V block (row kernel) or page (prefill kernel) met
+// so far. It follows a larger one, and one that lies more than 2^8 below it: what enters
+// as halves carries the ratio of the two, and bits below 2^-24 are lost. It stays within
+// 2^60 of the largest, vtop, where the sums are finite, and at a scale, 2^-100 or more.
+constexpr float kVSlack = 0x1p-8f;
+__device__ __forceinline__ bool vref_moves(float vref, float vs) { return vs > vref || vs < vref * kVSlack; }
+__device__ __forceinline__ float next_vref(float vref, float& vtop, float vs) {
+    vtop = fmaxf(vtop, vs);
+    return vref_moves(vref, vs) ? fmaxf(vs, fmaxf(vtop * 0x1p-60f, 0x1p-100f)) : vref;
+}
+
 // 2^x, about 2 units in the last place; 0 far below.
 __device__ __forceinline__ float ex2(float x) {
     float y;

@@ -15,7 +15,9 @@
 // 2^-29 of the row's largest value. An f32 row enters as two halves (value and
 // remainder, 22 bits together): a tile then holds 8 rows, their remainders in
 // the tile's other 8 rows, so the second half costs no further product. The
-// probabilities of f32 rows are split the same way.
+// probabilities of f32 rows are split the same way. Those of 16-bit rows enter as one
+// half, off by 2^-11 of themselves: no more than the output's own rounding (fp16;
+// bf16 2^-8), and a second half would cost as many products again.
 //
 // Bound by the cache's bytes: 24 rows over 300 to 32000 keys (40 / 10 heads of 128,
 // 0.91 GB) take 169 us, 5.4 TB/s or 83 % of the copy peak; 64 x 7 rows over 1000 to
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
         }
         float m[RR], l[RR];
         float o[NC][4][4];
-        float vref = 0.0f;   // scale of the accumulators: the largest V scale so far
+        float vref = 0.0f, vtop = 0.0f;   // scale of the accumulators (next_vref)
 #pragma unroll
         for (int r = 0; r < RR; r++) {
             m[r] = -INFINITY;
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
             }
             // reference of the maximum, and of the V scale
             float mx[RR];
-            bool move = vs > vref;
+            bool move = vref_moves(vref, vs);
 #pragma unroll
             for (int r = 0; r < RR; r++) {
                 mx[r] = fmaxf(fmaxf(s[r][0], s[r][1]), fmaxf(s[r][2], s[r][3]));
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                 move |= mx[r] > m[r] + kSlack || (m[r] == -INFINITY && mx[r] > m[r]);
             }
             if (__any_sync(0xffffffffu, move)) {
-                const float vnew = fmaxf(vs, vref);
+                const float vnew = next_vref(vref, vtop, vs);
                 const float vr = vref * pow2_inv(vnew);
                 vref = vnew;
 #pragma unroll

@@ -16,7 +16,7 @@
 //    come as 16-byte pieces (fl_kv8.h), a page ahead of their use, and go to one of
 //    two stages as halves: a K piece is two 16-byte chunks of two keys' rows; a V
 //    piece holds four keys of four dimensions, so V^T is written without a
-//    transposition. V is scaled by its block's scale over the largest so far (a power
+//    transposition. V is scaled by its block's scale over the accumulators' (next_vref; a power
 //    of two, in the multiply-add that removes the INT8 offset). Both tiles use it.
 //  - warp 12: one thread issues the products, S of the next page before P V of
 //    this, tile by tile, so that one tile's softmax runs beside the other's
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool ok = true;
             if (lane == 0 && n > 0) mb_arrive(&bar.q_full);
             const uint32_t tq = tmem + tile * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
-            float m = -INFINITY, l = 0.0f, vref = 0.0f;
+            float m = -INFINITY, l = 0.0f, vref = 0.0f, vtop = 0.0f;
             const int lim = ctx + (p.mask ? min(nb, p.ldm) : tok + 1);   // positions this row may see
             // dead rows read some row of the mask, to no effect
             const uint8_t* mrow = p.mask + (size_t)(live ? row : min(row0, p.rows - 1)) * p.ldm;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < n; j++) {
                 const uint32_t J = jb + j;
                 const float4 ks4 = next.k;
-                const float vs = vscale_max(next.v, k0 + j * kPageSize, ctx + nb);
+                const float vnew = next_vref(vref, vtop, vscale_max(next.v, k0 + j * kPageSize, ctx + nb));
                 next.load(p, bt, h, j + 1, n);
                 if (!warp_wait(&bar.s_full[J & 1], (J >> 1) & 1, tl.wait_clocks)) { ok = false; break; }
                 tc_after();
@@ -384,11 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const float vnew = fmaxf(vref, vs);
                 const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
                 if (j == 0) {
                     m = mx;
-                } else if (__any_sync(0xffffffffu, move || vnew > vref)) {
+                } else if (__any_sync(0xffffffffu, move || vnew != vref)) {
                     const float mn = fmaxf(m, mx);
                     const float al = m == -INFINITY ? 0.0f : ex2(m - mn);
                     m = mn;
@@ -519,10 +518,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             // V^T rows: dimension 32 c + 4 g + i, keys 16 blk + 4 t4 .. + 3; positions
             // behind the sequence may hold anything, an E4M3 NaN too
-            float vref = 0.0f;
+            float vref = 0.0f, vtop = 0.0f;
             auto write_v = [&](uint32_t st, int j, const float4& vs4) {
                 const int kb = k0 + j * kPageSize + blk * kKv8Block;
-                vref = fmaxf(vref, vscale_max(vs4, k0 + j * kPageSize, ctx + nb));
+                vref = next_vref(vref, vtop, vscale_max(vs4, k0 + j * kPageSize, ctx + nb));
                 const float vs = blk < 2 ? (blk ? vs4.y : vs4.x) : (blk == 2 ? vs4.z : vs4.w);
                 const float ratio = kb < ctx + nb ? vs * pow2_inv(vref) * kVUp : 0.0f;
                 const int left = ctx + nb - kb - 4 * t4;

@@ -243,7 +243,11 @@ int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, int rows
  * rows behind ldm, of a plan replayed from a graph, are not seen).
  * A row that sees nothing gives zeros. Rows behind the last planned one, and
  * behind `rows`, are left as they were. Products are taken with halves and
- * summed in 32 bits; f32 queries and their probabilities keep 22 bits. */
+ * summed in 32 bits: f32 queries and their probabilities as two halves (22 bits),
+ * those of 16-bit queries as one (11 bits). A probability far below the row's
+ * largest is off by at most 2^-24 of that, counted at the V scale of its block (in
+ * batches of many rows: of its page, where V itself keeps its codes down to 2^-20
+ * of the page's largest scale). */
 int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo, float scale,
                      const uint8_t* mask, int ldm, void* stream);
 

@@ -849,3 +849,63 @@ def test_attention_behind_a_replayed_plan(gpu, dtype, new):
     want, parts = p.m.attention(q1.double().cpu().numpy(), 0.125)
     assert (np.abs(out1.double().cpu().numpy() - want) <= attention_bound(dtype, want, parts, 64)).all()
     del g
+
+
+# ------------------------------------------------------------ V scales far apart
+def check_small_values(p, q, small, mask=None):
+    """Rows whose weight lies on keys with small V (at most `small`), beside keys of
+    far larger V without weight. The scale of a block (in the kernel for many rows, of
+    a page) is at least 2^-8 of the accumulators', so a probability's halves lose 2^-24
+    of its own block's V instead of the 2^-31 of the largest V that attention_bound counts."""
+    got = torch.full_like(q, 9.0)
+    p.c.attention(0, q, got, 1.0, None if mask is None else dev(mask, torch.uint8), stream=0)
+    want, (mag, smag, keys, vmax) = p.m.attention(q.double().cpu().numpy(), 1.0, mask)
+    assert np.abs(want).max() <= small
+    err = np.abs(got.double().cpu().numpy() - want)
+    tol = attention_bound(p.dtype, want, (mag, smag, keys, np.full_like(vmax, 2.0 ** 7 * small)), p.hd)
+    assert not np.isnan(err).any() and (err <= tol).all(), f"{(err / tol).max():.3g} x the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("far,new,unit", [(-12, 6, BLOCK), (-20, 6, BLOCK), (-40, 6, BLOCK), (-12, 200, BLOCK),
+                                          (-20, 200, PAGE), (-40, 200, PAGE)])
+def test_values_of_scales_far_apart(gpu, far, new, unit, dtype, type):
+    """Blocks (or pages) of keys with V near 1, which no row weighs (scores 60 lower:
+    2^-86), among others with V near 2^far, in changing order; few rows and many."""
+    rng = np.random.default_rng(-far)
+    p = Pair(gpu, heads=2, kv_heads=1, hd=64, dtype=dtype, type=type, max_rows=1200, max_ctx=1200, pages=100)
+    n = 1000
+    large = rng.random((n + new) // unit + 1) < 0.4
+    large[:3] = True, False, True
+    large[-3:] = False, True, False
+    large = np.repeat(large, unit)[:n + new]
+    k = rng.standard_normal((n + new, 1, 64)) * 0.3
+    k[:, :, 0] = np.where(large, -30.0, 30.0)[:, None]
+    v = rng.uniform(-1, 1, (n + new, 1, 64)) * np.where(large, 1.0, 2.0 ** far)[:, None, None]
+    k, v = (dev(x, torch.float32).to(getattr(torch, dtype)) for x in (k, v))
+    q = p.rows(rng, 2, new)
+    q[:, :, 0] = 1.0
+    p.plan([0], [n])
+    p.append(k[:n], v[:n])
+    p.plan([n], [new])
+    p.append(k[n:], v[n:])
+    check_small_values(p, q, 2.0 ** far)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", [-20, -40])
+@pytest.mark.parametrize("new,hidden", [(90, 2 * BLOCK), (200, PAGE)])
+def test_unseen_values_of_larger_scales(gpu, far, new, hidden):
+    """Large V in the first new rows, which the mask hides from every row."""
+    rng = np.random.default_rng(17)
+    p = Pair(gpu, heads=1, kv_heads=1, hd=64)
+    p.plan([0], [new])
+    k, v = rng.standard_normal((2, new, 1, 64))
+    v = np.clip(v, -1, 1) * np.where(np.arange(new) < hidden, 1.0, 2.0 ** far)[:, None, None]
+    p.append(dev(k, torch.float32), dev(v, torch.float32))
+    mask = (rng.random((new, new)) < 0.5).astype(np.uint8)
+    mask[:, :hidden] = 0
+    mask[:, -1] = 1
+    check_small_values(p, p.rows(rng, 1) * 0.3, 2.0 ** far, mask)
