@@ -34,6 +34,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "fl_common.cuh"
 #include "fl_kv8.h"
@@ -45,6 +46,7 @@ namespace fl {
 namespace {
 
 __device__ int g_kv8_error = 0;
+std::atomic<bool> g_kv8_launched{false};   // the kernel was launched (or captured) in this process
 
 constexpr int kRows = 128;               // query rows of a tile
 constexpr int kPair = kKv8Long;          // of a CTA's two tiles
@@ -695,6 +697,7 @@ cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int c
     const int es = p.dtype == FL_F32 ? 4 : 2;
     const int vec = ((uintptr_t)p.q & 15) == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldq * es % 16 == 0 &&
                     p.ldo * es % 16 == 0;
+    g_kv8_launched.store(true, std::memory_order_relaxed);
     return with_kernel(p.head_dim, p.type, p.dtype, [&](auto* k, int smem) {
         k<<<ctas, kThreads, smem, s>>>(p, tl, vec);
         return cudaGetLastError();
@@ -703,6 +706,7 @@ cudaError_t launch_kv8_prefill(const Kv8AttnParams& p, const Kv8Tiles& tl, int c
 
 int take_kv8_error() {
     int v = 0;
+    if (!g_kv8_launched.load(std::memory_order_relaxed)) return 0;   // no wait could give up: no copy
     if (cudaMemcpyFromSymbol(&v, g_kv8_error, sizeof(int)) != cudaSuccess) return -1;
     if (v) {
         const int z = 0;
