@@ -909,3 +909,101 @@ def test_unseen_values_of_larger_scales(gpu, far, new, hidden):
     mask[:, :hidden] = 0
     mask[:, -1] = 1
     check_small_values(p, p.rows(rng, 1) * 0.3, 2.0 ** far, mask)
+
+
+# -------------------------------------------- CTAs that take one tile after another
+def ragged(kind, rng):
+    """heads, kv_heads, hd, cached lengths, new rows: more (tile, kv head) pairs than
+    CTAs, shared as whole tiles or, beside a few long sequences, as equal parts."""
+    if kind == "rows-whole":
+        return 32, 32, 32, rng.integers(0, 200, 48), rng.integers(1, 4, 48)
+    if kind == "rows-parts":
+        return 32, 16, 64, np.r_[rng.integers(0, 100, 60), 7000, 3000], rng.integers(1, 9, 62)
+    if kind == "chunks-whole":
+        return 16, 8, 64, rng.integers(0, 300, 24), rng.integers(97, 200, 24)
+    if kind == "chunks-parts":
+        return 16, 8, 64, np.r_[6000, rng.integers(0, 100, 20)], rng.integers(97, 150, 21)
+    return 16, 8, 128, np.r_[rng.integers(0, 700, 20), 5000], np.r_[rng.integers(97, 150, 9), rng.integers(1, 40, 12)]
+
+
+def check_in_bulk(p, q, mask=None):
+    """check_attention with the model's formulas as 64-bit products on the GPU."""
+    got = torch.full_like(q, 9.0)
+    p.c.attention(0, q, got, None, None if mask is None else dev(mask, torch.uint8), stream=0)
+    scale, r = float(np.float32(p.hd ** -0.5)), 0
+    mk = None if mask is None else dev(mask, torch.bool)
+    for b, m in enumerate(p.m.new):
+        if not m:
+            continue
+        n, g = p.m.ctx[b] + m, p.H // p.Hk
+        K, V = (dev(p.m.values(x, b), torch.float64) for x in "kv")
+        x = q[r:r + m].double().view(m, p.Hk, g, p.hd)
+        see = torch.arange(n, device="cuda")[None] <= p.m.ctx[b] + torch.arange(m, device="cuda")[:, None]
+        if mk is not None:
+            see[:, p.m.ctx[b]:] = mk[r:r + m, :m]
+        see, any_ = see[:, None, None], see.any(1)[:, None, None]
+        S = torch.einsum("mhgd,nhd->mhgn", x, K) * scale
+        w = torch.where(any_[..., None], torch.where(see, S, -np.inf), 0.0).softmax(-1) * see
+        want = torch.einsum("mhgn,nhd->mhgd", w, V)
+        mag = torch.einsum("mhgn,nhd->mhgd", w, V.abs())
+        smag = (torch.einsum("mhgd,nhd->mhgn", x.abs(), K.abs()) * see).amax(-1) * scale
+        vmax = (V.abs().amax(-1).T[:, None] * see).amax(-1)
+        keys = see.sum(-1).clamp(min=1)
+        full = lambda a: a.expand(m, p.Hk, g).reshape(m, p.H).cpu().numpy()
+        want, mag = (a.reshape(m, p.H, p.hd).cpu().numpy() for a in (want, mag))
+        err = np.abs(got[r:r + m].double().cpu().numpy() - want)
+        tol = attention_bound(p.dtype, want, (mag, full(smag), full(keys), full(vmax)), p.hd)
+        assert not np.isnan(err).any() and (err <= tol).all(), f"{(err / np.maximum(tol, 1e-300)).max():.3g} x the bound"
+        r += m
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,type", [("float32", "int8"), ("bfloat16", "e4m3"), ("float16", "int8")])
+@pytest.mark.parametrize("kind", ["rows-whole", "rows-parts", "chunks-whole", "chunks-parts", "both"])
+def test_more_tiles_than_ctas(gpu, kind, dtype, type):
+    """Barriers, rings and workspaces carried from tile to tile within a CTA, with and
+    without a mask; the same call again gives the same bits."""
+    rng = np.random.default_rng(18)
+    H, Hk, hd, ctx, new = ragged(kind, rng)
+    pages = int((-(-(ctx + new) // PAGE)).sum())
+    p = Pair(gpu, heads=H, kv_heads=Hk, hd=hd, dtype=dtype, type=type, pages=pages, max_seqs=len(ctx),
+             max_rows=int(max(ctx.sum(), new.sum())), max_ctx=int((ctx + new).max()))
+    p.plan([0] * len(ctx), ctx.tolist(), check=False)
+    p.append(p.rows(rng, Hk, scale=2.0), p.rows(rng, Hk))
+    p.plan(ctx.tolist(), new.tolist(), check=False)
+    p.append(p.rows(rng, Hk, scale=2.0), p.rows(rng, Hk))
+    q = p.rows(rng, H)
+    first = check_in_bulk(p, q)
+    for _ in range(5):
+        out = torch.full_like(q, 9.0)
+        p.c.attention(0, q, out, hd ** -0.5, stream=0)
+        assert torch.equal(out, first)
+    mask = (rng.random((int(new.sum()), int(new.max()))) < 0.5).astype(np.uint8)
+    check_in_bulk(p, q, mask)
+    p.c.attention(0, q, out, stream=0)
+    assert torch.equal(out, first)
+    assert gpu.fl_cuda_sync() == 0
+
+
+@pytest.mark.gpu
+def test_plans_refused_in_the_life_of_a_batch(gpu):
+    """Steps of a running batch that lack pages, that have too many rows, and that go
+    through, all of them among the steps."""
+    rng = np.random.default_rng(1)
+    p = Pair(gpu, pages=20, max_seqs=9, max_rows=300, max_ctx=500)
+    pos, seen = np.zeros(9, int), []
+    for step in range(60):
+        new = np.minimum(rng.integers(0, 40, 9), 512 - pos)
+        new[rng.random(9) < 0.1] = -1
+        if step % 6 == 3:
+            new[rng.integers(9)] = 260 if step % 4 == 1 else 150
+        p.plan(pos.tolist(), new.tolist(), max_new=260)
+        seen.append(p.m.status)
+        if p.m.status == 0:
+            pos = np.where(new < 0, 0, pos + np.maximum(new, 0))
+        elif p.m.status > 0:                     # a scheduler makes room
+            pos[:3] = 0
+            p.plan(pos.tolist(), [-1] * 3 + [0] * 6, max_new=260)
+            assert p.m.status == 0
+    assert 0 in seen and -1 in seen and max(seen) > 0
