@@ -72,6 +72,7 @@ struct fl_kv8 {
     float* part[2] = {};        // [2 parts][rows of a tile][head_dim] partial outputs
     float2* part_ml[2] = {};    // [2 parts][rows of a tile] (maximum, sum)
     int* part_cnt[2] = {};      // [parts] arrivals, zero between launches
+    float4* fold = nullptr;     // [parts[1]][head_dim / 4][kKv8Long] sums over a CTA's earlier pages
 };
 
 namespace fl {
@@ -96,6 +97,7 @@ struct Kv8Tiles {
     float* part;
     float2* part_ml;
     int* part_cnt;
+    float4* fold;        // the prefill kernel's sums over earlier pages
     // the prefill kernel's bounded waits; fail_at > 0: the issuing thread of CTA
     // fail_cta stops before its fail_at-th group of products, as if a wait had run out
     long long wait_clocks;

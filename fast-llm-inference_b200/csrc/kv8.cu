@@ -630,6 +630,7 @@ int create(fl_kv8* h) {
         FL_CHECK(alloc(h, &h->part_ml[i], rows, false));
         FL_CHECK(alloc(h, &h->part_cnt[i], h->parts[i], true));
     }
+    FL_CHECK(alloc(h, &h->fold, (size_t)h->parts[1] * (c.head_dim / 4) * kKv8Long, false));
     kv8_reset_kernel<<<64, 256>>>(t, c.pages, c.max_seqs);
     FL_CHECK_CUDA(cudaGetLastError());
     FL_CHECK_CUDA(cudaDeviceSynchronize());
@@ -866,7 +867,7 @@ int attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t
     Kv8Tiles tl[2];
     for (int i = 0; i < 2; i++)
         tl[i] = Kv8Tiles{i, h->t.tile_start[i], h->t.work_start[i], h->part[i], h->part_ml[i], h->part_cnt[i],
-                         wait.clocks, wait.fail_cta, wait.fail_at};
+                         h->fold, wait.clocks, wait.fail_cta, wait.fail_at};
     FL_CHECK_CUDA(launch_kv8_attention(p, tl[0], h->parts[0], s));
     // The plan that this call will find may be a replayed one, unless both are in one capture
     const bool own_plan = h->plan_capture && h->plan_capture == capture_of(s);

@@ -19,6 +19,11 @@
 // half, off by 2^-11 of themselves: no more than the output's own rounding (fp16;
 // bf16 2^-8), and a second half would cost as many products again.
 //
+// A product drops the bits of its sums below 2^-24, towards zero, so that sums over n
+// blocks of a sign fall short by about n 2^-25 (30 k keys: 1.6e-5). f32 rows therefore add
+// each block's products, rounded, to sums of their own; 16-bit rows, whose outputs round
+// coarser, sum up in the products.
+//
 // Bound by the cache's bytes: 24 rows over 300 to 32000 keys (40 / 10 heads of 128,
 // 0.91 GB) take 169 us, 5.4 TB/s or 83 % of the copy peak; 64 x 7 rows over 1000 to
 // 1500 keys (32 heads of 96, 0.53 GB) 111 us, 73 %. Loads straight into registers
@@ -44,6 +49,17 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The products alone, of rows 0 - 7 and 8 - 15 together, added to d rounded.
+__device__ __forceinline__ void mma16816_rounded(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    float x[4];
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    d[0] += x[0] + x[2];
+    d[1] += x[1] + x[3];
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -259,10 +275,6 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                         for (int j = 0; j < 4; j++) {
                             o[c][j][2 * r] *= f;
                             o[c][j][2 * r + 1] *= f;
-                            if constexpr (F32) {
-                                o[c][j][2] *= f;
-                                o[c][j][3] *= f;
-                            }
                         }
                 }
             }
@@ -294,7 +306,8 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                 for (int j = 0; j < 4; j++) {
                     uint32_t b0, b1;
                     codes_to_halves<E4M3>(vw[j], b0, b1);
-                    mma16816(o[c][j], pa, b0, b1);
+                    if constexpr (F32) mma16816_rounded(o[c][j], pa, b0, b1);
+                    else mma16816(o[c][j], pa, b0, b1);
                 }
             }
         }
@@ -318,7 +331,7 @@ __global__ void __launch_bounds__(kAW * 32, 3) kv8_attention_kernel(const Kv8Att
                     float* vp = reinterpret_cast<float*>(&v);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        vp[j] = (F32 ? o[c][j][e] + o[c][j][2 + e] : o[c][j][2 * r + e]) * f;
+                        vp[j] = o[c][j][2 * r + e] * f;
                     *reinterpret_cast<float4*>(&o_s[warp][g + 8 * r][c * 32 + 8 * t4 + 4 * e]) = v;
                 }
         }

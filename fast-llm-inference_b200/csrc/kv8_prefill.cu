@@ -24,6 +24,13 @@
 //    instead of the figure below.)
 // f32 rows take two halves for Q and for P (22 bits): twice the products.
 //
+// Every product drops the bits of its sums below 2^-24, towards zero: over n products
+// sums of one sign fall short by about n 2^-25. That is 1.4e-4 for f32 rows over 30 k
+// keys, so their O goes to sums rounded to nearest, in the workspace, every 4 pages (32
+// products, remainders first while the sums are small): f32 chunks of the sizes below
+// take 0.97 ms, without 0.82. 16-bit rows have half the products and round coarser:
+// they keep what is lost, about 2^-16 for each 4096 keys.
+//
 // Bound by the issue of the products, about 80 clocks each: 24 per page and pair of
 // tiles, 2500 of some 3900 clocks; then by the softmax warps' chain per page (2700).
 // Prompt chunks of 0.8 to 2 k rows behind 0 to 6 k keys (32 / 8 heads of 128, 0.34
@@ -229,6 +236,13 @@ struct Layout {
     static constexpr int kBytes = kV + 2 * kVStage + 1024;
 };
 
+// A row's sums over the pages before the last fold: dimensions 4 d .. 4 d + 3 at d
+// kPair, so that a warp's accesses are whole lines.
+template <int HD>
+__device__ __forceinline__ float4* fold_row(const Kv8Tiles& tl) {
+    return tl.fold + (size_t)blockIdx.x * (HD / 4) * kPair + threadIdx.x;
+}
+
 // What a tile's warps and the issuing thread signal to each other. p_full is by
 // buffer, as s_full: a warp may write the next page's P before a slower one has
 // written this page's, and the barrier must not count its arrival for that one.
@@ -242,6 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool F32 = DT == FL_F32;
     typedef Layout<HD, F32> L;
     constexpr int NC = HD / 32;
+    constexpr int kFold = 4;   // pages, of f32 rows
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) TileBars bars[2];
     __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
@@ -336,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0 && n > 0) mb_arrive(&bar.q_full);
             const uint32_t tq = tmem + tile * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
             float m = -INFINITY, l = 0.0f, vref = 0.0f, vtop = 0.0f;
+            float mf = -INFINITY, vf = 0.0f;   // reference and scale of the rounded sums
             const int lim = ctx + (p.mask ? min(nb, p.ldm) : tok + 1);   // positions this row may see
             // dead rows read some row of the mask, to no effect
             const uint8_t* mrow = p.mask + (size_t)(live ? row : min(row0, p.rows - 1)) * p.ldm;
@@ -389,6 +405,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const bool move = mx > m + kSlack || (m == -INFINITY && mx > m);
                 if (j == 0) {
                     m = mx;
+                } else if (F32 && j % kFold == 0) {
+                    // O to the rounded sums, in O's units; the next product begins it anew
+                    if (!warp_wait(&bar.pv_done, (J - 1) & 1, tl.wait_clocks)) { ok = false; break; }
+                    tc_after();
+                    const float g = mf == -INFINITY ? 0.0f : ex2(mf - m) * (vf * pow2_inv(vref));
+                    float4* sum = fold_row<HD>(tl);
+#pragma unroll 1
+                    for (int c = 0; c < NC; c++) {   // the loads of 32 dimensions at once
+                        float o[32];
+                        float4 b[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            b[i] = j == kFold ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(sum + (8 * c + i) * kPair);
+                        tmem_ld32(tq + 128 + 32 * c, o);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            __stcg(sum + (8 * c + i) * kPair,
+                                   make_float4(__fmaf_rn(b[i].x, g, o[4 * i]), __fmaf_rn(b[i].y, g, o[4 * i + 1]),
+                                               __fmaf_rn(b[i].z, g, o[4 * i + 2]), __fmaf_rn(b[i].w, g, o[4 * i + 3])));
+                    }
+                    mf = m;
+                    vf = vref;
+                    m = fmaxf(m, mx);
+                    l *= mf == -INFINITY ? 0.0f : ex2(mf - m);
                 } else if (__any_sync(0xffffffffu, move || vnew != vref)) {
                     const float mn = fmaxf(m, mx);
                     const float al = m == -INFINITY ? 0.0f : ex2(m - mn);
@@ -459,6 +500,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_after();
                 const size_t slot = 2 * (size_t)blockIdx.x + (it.split == 0);
                 const float g = l != 0.0f ? __fdiv_rn(vref * (1.0f / kVUp), l) : 0.0f;
+                const bool folded = F32 && n > kFold;
+                const float gf = mf == -INFINITY ? 0.0f : ex2(mf - m) * (vf * pow2_inv(vref));
+                const float4* sum = fold_row<HD>(tl);
 #pragma unroll 1
                 for (int c = 0; c < NC; c++) {
                     float o[32];
@@ -469,6 +513,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
+                        if (folded) {
+                            const float4 b = __ldcg(sum + (8 * c + i / 4) * kPair);
+                            o[i] = __fmaf_rn(b.x, gf, o[i]);
+                            o[i + 1] = __fmaf_rn(b.y, gf, o[i + 1]);
+                            o[i + 2] = __fmaf_rn(b.z, gf, o[i + 2]);
+                            o[i + 3] = __fmaf_rn(b.w, gf, o[i + 3]);
+                        }
                         float v[4];
 #pragma unroll
                         for (int k = 0; k < 4; k++) v[k] = n > 0 && l != 0.0f ? o[i + k] * g : 0.0f;
@@ -575,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (fail && --fail == 0) return false;
                 tc_after();
 #pragma unroll
-                for (int q = 0; q < L::kParts; q++)
+                for (int q = L::kParts - 1; q >= 0; q--)   // the remainders first, while the sums are small
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++)
                         umma_f16<kPageSize>(tmem + tile * 256 + (T & 1) * 64,
@@ -583,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                        (k >> 2) * (kRows * 128) + (k & 3) * 32),
                                             desc_sw128(smem + L::kK + (J & 1) * L::kKStage +
                                                        (k >> 2) * (kPageSize * 128) + (k & 3) * 32),
-                                            q + k > 0);
+                                            q < L::kParts - 1 || k > 0);
                 umma_commit(&bars[tile].s_full[T & 1]);
                 if (tile == nt - 1) umma_commit(&k_empty[J & 1]);
                 return true;
@@ -596,11 +647,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (fail && --fail == 0) return false;
                 tc_after();
 #pragma unroll
-                for (int q = 0; q < L::kParts; q++)
+                for (int q = L::kParts - 1; q >= 0; q--)
 #pragma unroll
                     for (int k = 0; k < kPageSize / 16; k++)
                         umma_f16_ta<HD>(tmem + tile * 256 + 128, tmem + tile * 256 + (T & 1) * 64 + q * 16 + (k >> 1) * 32 + (k & 1) * 8,
-                                        desc_sw128(smem + L::kV + (J & 1) * L::kVStage + k * 32), j > 0 || q + k > 0);
+                                        desc_sw128(smem + L::kV + (J & 1) * L::kVStage + k * 32), (F32 ? j % kFold : j) > 0 || q < L::kParts - 1 || k > 0);
                 umma_commit(&bars[tile].pv_done);
                 if (tile == nt - 1) umma_commit(&v_empty[J & 1]);
                 return true;

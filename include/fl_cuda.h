@@ -247,7 +247,8 @@ int fl_kv8_append(fl_kv8_t* h, int layer, const void* k, const void* v, int rows
  * those of 16-bit queries as one (11 bits). A probability far below the row's
  * largest is off by at most 2^-24 of that, counted at the V scale of its block (in
  * batches of many rows: of its page, where V itself keeps its codes down to 2^-20
- * of the page's largest scale). */
+ * of the page's largest scale). Sums of 16-bit rows fall short by up to 2^-16 for
+ * each 4096 keys where they are of one sign; those of f32 rows are rounded. */
 int fl_kv8_attention(fl_kv8_t* h, int layer, const void* q, void* out, int rows, size_t ldq, size_t ldo, float scale,
                      const uint8_t* mask, int ldm, void* stream);
 

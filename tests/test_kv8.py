@@ -1007,3 +1007,42 @@ def test_plans_refused_in_the_life_of_a_batch(gpu):
             p.plan(pos.tolist(), [-1] * 3 + [0] * 6, max_new=260)
             assert p.m.status == 0
     assert 0 in seen and -1 in seen and max(seen) > 0
+
+
+# --------------------------------------------------------- sums over many keys
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["int8", "e4m3"])
+@pytest.mark.parametrize("seqs,kv_heads,hd,ctx,new", [(12, 40, 32, 30000, 1), (1, 40, 32, 30000, 1024), (1, 20, 128, 20000, 2048)])
+def test_sums_over_many_keys_do_not_drift(gpu, seqs, kv_heads, hd, ctx, new, type):
+    """f32 rows over tens of thousands of keys that one CTA takes in a row, V positive:
+    sums that drop the bits below 2^-24 at each of n products fall short by about
+    n 2^-25; rounded ones do not fall short on average. 2^-20 is 32 steps of 2^-25 left
+    to the products of a few blocks, twice over. One value is off by at most that,
+    2^-22 for its probabilities' halves, 2^-24 for each 16 keys, and the scores' errors,
+    2^-20 of scores below 8."""
+    n = ctx + new
+    c = flb200.KV8Cache(gpu, layers=1, heads=kv_heads, kv_heads=kv_heads, head_dim=hd, pages=seqs * -(-n // PAGE),
+                        max_seqs=seqs, max_rows=max(ctx, seqs * new), max_ctx=n, type=type, dtype="float32")
+    g = torch.Generator(device="cuda").manual_seed(19)
+    v = torch.rand((n, kv_heads, hd), generator=g, device="cuda") * 0.5 + 0.5
+    k = torch.randn((n, kv_heads, hd), generator=g, device="cuda")
+    for b in range(seqs):
+        c.plan(dev([0] * seqs), dev([ctx if i == b else 0 for i in range(seqs)]), ctx, stream=0)
+        c.append(0, k[:ctx], v[:ctx], stream=0)
+    c.plan(dev([ctx] * seqs), dev([new] * seqs), new, stream=0)
+    c.append(0, k[ctx:].repeat(seqs, 1, 1), v[ctx:].repeat(seqs, 1, 1), stream=0)
+    q = torch.randn((new, kv_heads, hd), generator=g, device="cuda").repeat(seqs, 1, 1)
+    out = torch.full_like(q, 9.0)
+    c.attention(0, q, out, stream=0)
+    gk, gv = (torch.empty((seqs * n, kv_heads, hd), device="cuda") for _ in range(2))
+    c.gather(0, gk, gv, stream=0)
+    hide = torch.arange(n, device="cuda") > ctx + torch.arange(new, device="cuda")[:, None]
+    scale, rel = float(np.float32(hd ** -0.5)), []
+    for h in range(0, kv_heads, 3):
+        S = q[:new, h].double() @ gk[:n, h].double().T * scale
+        assert S.abs().max() < 8
+        want = S.masked_fill_(hide, -np.inf).softmax(1) @ gv[:n, h].double()
+        rel.append((out[:, h].view(seqs, new, hd).double() - want) / want)
+    rel = torch.stack(rel)
+    assert abs(float(rel.mean())) <= 2.0 ** -20
+    assert float(rel.abs().max()) <= 2.0 ** -20 + 2.0 ** -22 + n / 16 * 2.0 ** -24 + 2.0 ** -17
