@@ -29,10 +29,10 @@ constexpr int kSmSeqs = 1024;   // sequences whose starts shared memory holds
 
 // Packed query rows of a sequence (new rows x heads per kv head) from which the
 // prefill kernel takes it. 128 / 188 rows in 16 bits: 4 sequences x 3700 keys (10 kv
-// heads x 128) 71 / 93 us, the row kernel 68 / 94; 1 x 16 k 84 / 112, 69 / 91; 32 x 1000
-// 120 / 157, 155 / 229. f32, whose products are twice as many in either, at 96 rows (32
-// heads x 96): 116, 133 and 309 us, the row kernel 187, 183 and 490; at 64 rows 112, 128
-// and 289 to 129, 128 and 316, but 32 to 15 at one sequence of 600 keys.
+// heads x 128) 71 / 90 us, the row kernel 77 / 103; 1 x 16 k 82 / 107, 77 / 101; 32 x 1000
+// 127 / 157, 169 / 251; one of 600 keys 33 / 43, 17 / 19. f32 (32 heads x 96) at 96 rows: 163,
+// 175, 423 and 43 us, the row kernel 195, 193, 502 and 16; at 64 rows 159, 172, 401 and 43 to
+// 135, 135, 325 and 16.
 #ifndef FL_KV8_LONG_MIN
 #define FL_KV8_LONG_MIN 192
 #endif
