@@ -25,8 +25,8 @@
 // coarser, sum up in the products.
 //
 // Bound by the cache's bytes: 24 rows over 300 to 32000 keys (40 / 10 heads of 128,
-// 0.91 GB) take 169 us, 5.4 TB/s or 83 % of the copy peak; 64 x 7 rows over 1000 to
-// 1500 keys (32 heads of 96, 0.53 GB) 111 us, 73 %. Loads straight into registers
+// 0.91 GB) take 172 to 185 us, 75 to 81 % of the copy peak; 64 x 7 f32 rows over 1000 to
+// 1500 keys (32 heads of 96, 0.53 GB) 114 us, 71 %. Loads straight into registers
 // took 315 and 142 us: a warp waited for each block. Each warp takes one block of
 // every page, so that nothing is shared before the tile's end.
 #include <math.h>

@@ -34,7 +34,7 @@
 // Bound by the issue of the products, about 80 clocks each: 24 per page and pair of
 // tiles, 2500 of some 3900 clocks; then by the softmax warps' chain per page (2700).
 // Prompt chunks of 0.8 to 2 k rows behind 0 to 6 k keys (32 / 8 heads of 128, 0.34
-// TFLOP) take 0.85 ms, 0.4 PFLOP/s; the row kernel takes 2.47 ms.
+// TFLOP) take 0.84 ms, 0.4 PFLOP/s; the row kernel takes 2.47 ms.
 //
 // Waits are bounded (kKv8WaitClocks, about 2 s); on expiry the CTA raises an error word,
 // stops, waits (bounded) for all products that it issued, frees TMEM and exits.

@@ -12,11 +12,12 @@
 // with all at once. Counts and masses share one 64-bit word (44 bits of mass).
 // The draw is a prefix sum in token order: over the warps, each of which holds
 // a contiguous piece of the row, then within the one the target falls into.
-// Bound by instructions: about 25 a token for its weight, 3 for each of about
-// nine passes a threshold; few warps with much work each, because what a pass costs
-// apart from that are the warps' reductions (32 tokens a thread of 1024 took 85 us
-// where this takes 74: 448 rows of 32064 with mixed rules). One row takes 17 us, 61
-// rows of 128011 in 16 bits 112.
+// 448 rows of 32064 with mixed rules take 73 us, of which instructions are about 31
+// (25 a token for its weight, 3 for each of about 18 passes): one CTA fills an SM's
+// registers, so that nothing runs while its warps reduce and meet, and 448 rows are 3.03
+// waves. Few warps with much work each, because a pass costs apart from that
+// the warps' reductions (32 tokens a thread of 1024 took 85 us). One row takes 18 us
+// and 61 rows of 128011 in 16 bits 104, most of it cluster barriers.
 #include <float.h>
 #include <limits.h>
 
